@@ -341,7 +341,11 @@ int ugc_lookup_unique(ugc_ctx* ctx, int replica_id, const void* keys, int key_by
  * bytes and the tables 16-byte aligned (UGC_ERR_UNSUPPORTED otherwise).  Ordered against a
  * refresh like every lookup.  The reference has no such call: its applications hand the rows
  * to the model, which pools them (example/dlr/main.py: `combiner`). */
-typedef enum { UGC_ELEM_F32 = 0, UGC_ELEM_F16 = 1 } ugc_elem_type;
+typedef enum {
+  UGC_ELEM_F32 = 0,
+  UGC_ELEM_F16 = 1,
+  UGC_ELEM_BF16 = 2 /* routing and adapters only: the pooled lookup refuses it */
+} ugc_elem_type;
 typedef enum { UGC_POOL_SUM = 0, UGC_POOL_MEAN = 1 } ugc_pool_mode;
 int ugc_lookup_pool(ugc_ctx* ctx, int replica_id, const void* keys, int key_bytes, size_t n_keys,
                     const int64_t* offsets, size_t n_bags, size_t bag_size, int elem_type, int mode,
@@ -408,6 +412,80 @@ int ugc_hotness_read(ugc_ctx* ctx, int replica_id, uint32_t* counts_out, int res
  * ids by descending count, ties by ascending id; rank_freqs = their counts.  Replaces
  * FreqRecorder::Sort (coll_cache_lib/freq_recorder.cc:207-274). */
 int ugc_rank_hotness(uint64_t num_total_item, const uint32_t* counts, uint32_t* rank_ids, uint32_t* rank_freqs);
+
+/* -- routing: tokens grouped by what serves them -------------------------------------------- */
+/* What a model does with rows next: tokens go to the experts, or get the adapters, that ids name.
+ * The batch is planned once; every layer that uses the same ids uses the plan.  No reference
+ * counterpart.  These calls belong to no context: they work on `device_id` (and leave the caller's
+ * current device as it was), allocate nothing, keep nothing between calls and only enqueue work on
+ * `stream`, so any number of them may run at once on different streams, and all may be captured
+ * into a graph.  All pointers are device memory of that GPU; unless said otherwise no output may
+ * overlap an input.
+ *
+ * ugc_route_plan: a stable counting sort of n = n_tokens * k ids (int32 or int64; token t's choices
+ * are ids[t*k .. t*k+k)) into n_groups groups (at most UGC_ROUTE_MAX_GROUPS; n at most 2^28):
+ *   offsets[g]    place where group g starts in `order`, n_groups + 1 entries: offsets[n_groups] is
+ *                 the number of ids inside the groups, called `routed` below;
+ *   order[p]      index (t*k + j) of the id at place p: group by group, ascending inside a group;
+ *                 the ids outside [0, n_groups) (dropped choices, padding) come behind `routed`,
+ *                 ascending too, so that `order` is always a permutation of 0 .. n-1;
+ *   position[i]   place of id i in `order`, -1 for an id outside the groups.
+ * workspace: ugc_route_plan_workspace bytes (may be 0, then NULL will do), 4-byte aligned, free
+ * again when the call's work on the stream is done. */
+#define UGC_ROUTE_MAX_GROUPS 1024
+int ugc_route_plan_workspace(size_t n_tokens, size_t k, int n_groups, size_t* bytes);
+int ugc_route_plan(int device_id, const void* ids, int id_bytes, size_t n_tokens, size_t k, int n_groups,
+                   int32_t* offsets, int32_t* order, int32_t* position, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* The rows' way to their groups and back, and the gradients of both.  `x`, `y`, `dx`, `dy` are rows
+ * of tokens, n_tokens x dim; `rows`, `out`, `dout`, `drows` rows in the plan's order, n_tokens * k x
+ * dim; strides count elements from row to row (at least dim; rows themselves are contiguous); all of
+ * one ugc_elem_type.  weights / dweights: fp32, n_tokens x k, contiguous.  `position` and `routed`
+ * (the address of offsets[n_groups]) come from the plan.
+ *
+ *   dispatch       out[position[t,j]] = weights[t,j] * x[t]          (weights NULL: copied)
+ *   dispatch_grad  dx[t] = sum_j weights[t,j] * dout[position[t,j]]  (weights NULL: summed)
+ *                  dweights[t,j] = <x[t], dout[position[t,j]]>       (only if dweights is given)
+ *   combine        y[t] = sum_j weights[t,j] * rows[position[t,j]]   (weights NULL: summed)
+ *   combine_grad   drows[position[t,j]] = weights[t,j] * dy[t]       (weights NULL: copied)
+ *                  dweights[t,j] = <dy[t], rows[position[t,j]]>      (only if dweights is given)
+ *
+ * Sums and products are fp32, the choices of a token added in their order by fused multiply-adds,
+ * one rounding at the end; results do not depend on the launch.  A choice whose position is -1 (or
+ * outside the rows) adds nothing, its row is not read and its dweights are 0; a token without any
+ * choice gets zeros.  Rows of `out` and `drows` from `routed` on, which no choice takes, are zeroed;
+ * routed NULL: left as they were.  x / rows may be NULL in the gradients if dweights is. */
+int ugc_route_dispatch(int device_id, int elem_type, const void* x, int64_t x_stride, const float* weights,
+                       const int32_t* position, const int32_t* routed, size_t n_tokens, size_t k, size_t dim,
+                       void* out, int64_t out_stride, void* stream);
+int ugc_route_dispatch_grad(int device_id, int elem_type, const void* dout, int64_t dout_stride, const void* x,
+                            int64_t x_stride, const float* weights, const int32_t* position, size_t n_tokens,
+                            size_t k, size_t dim, void* dx, int64_t dx_stride, float* dweights, void* stream);
+int ugc_route_combine(int device_id, int elem_type, const void* rows, int64_t rows_stride, const float* weights,
+                      const int32_t* position, size_t n_tokens, size_t k, size_t dim, void* y, int64_t y_stride,
+                      void* stream);
+int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t dy_stride, const void* rows,
+                           int64_t rows_stride, const float* weights, const int32_t* position,
+                           const int32_t* routed, size_t n_tokens, size_t k, size_t dim, void* drows,
+                           int64_t drows_stride, float* dweights, void* stream);
+
+/* Low-rank adapters of many requests at once, beside a projection that all requests share:
+ *   out[t] = base[t] + scale[a] * (x[t] down[a]^T) up[a]^T,   a = group of token t in the plan (k = 1);
+ * a token without a group: out[t] = base[t].  base, out: n_tokens x out_dim; x: n_tokens x dim;
+ * down[a]: rank x dim, up[a]: out_dim x rank, each contiguous, adapters down_stride / up_stride
+ * elements apart -- so a row of an adapter table looked up through the cache can hold both, and the
+ * `inverse` of ugc_lookup_unique is the plan's ids.  scale: fp32 per adapter, or NULL for 1.
+ * out may be base itself (same stride); other overlaps are not allowed.  fp16 and bf16, rank at most
+ * UGC_ADAPTER_MAX_RANK; 16-byte aligned addresses and strides, dims and ranks in multiples of 8
+ * elements take the fast loads.  Sums are fp32; the rank products enter the second product as two
+ * 16-bit terms (16 significand bits or more). */
+#define UGC_ADAPTER_MAX_RANK 128
+int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x,
+                    int64_t x_stride, const void* down, int64_t down_stride, const void* up, int64_t up_stride,
+                    const float* scale, const int32_t* offsets, const int32_t* order, size_t n_tokens,
+                    int n_groups, size_t rank, size_t dim, size_t out_dim, void* out, int64_t out_stride,
+                    void* stream);
 
 /* -- introspection --------------------------------------------------------------------- */
 int ugc_stats(ugc_ctx* ctx, int replica_id, ugc_stats_t* out);

@@ -142,6 +142,7 @@ _lib = None
 
 # name -> (restype, argtypes); every symbol include/ugache_b200.h declares
 _P, _I, _U64, _SZ, _D = C.c_void_p, C.c_int, C.c_uint64, C.c_size_t, C.c_double
+_I64 = C.c_int64
 SIGNATURES = {
     "ugc_abi_sizes": (_I, [C.POINTER(C.c_uint32 * 5)]),
     "ugc_version": (C.c_char_p, []),
@@ -177,6 +178,14 @@ SIGNATURES = {
     "ugc_record": (_I, [_P, _I, _P, _I, _SZ, _P]),
     "ugc_hotness_read": (_I, [_P, _I, _P, _I, _P]),
     "ugc_rank_hotness": (_I, [_U64, _P, _P, _P]),
+    "ugc_route_plan_workspace": (_I, [_SZ, _SZ, _I, C.POINTER(_SZ)]),
+    "ugc_route_plan": (_I, [_I, _P, _I, _SZ, _SZ, _I, _P, _P, _P, _P, _SZ, _P]),
+    "ugc_route_dispatch": (_I, [_I, _I, _P, _I64, _P, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P]),
+    "ugc_route_dispatch_grad": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P, _P]),
+    "ugc_route_combine": (_I, [_I, _I, _P, _I64, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P]),
+    "ugc_route_combine_grad": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P, _P]),
+    "ugc_adapter_add": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _SZ, _I, _SZ, _SZ, _SZ, _P,
+                             _I64, _P]),
     "ugc_stats": (_I, [_P, _I, C.POINTER(Stats)]),
     "ugc_get_tuning": (_I, [_P, _I, C.POINTER(Tuning)]),
     "ugc_set_tuning": (_I, [_P, _I, C.POINTER(Tuning)]),
@@ -246,7 +255,9 @@ def fast():
                               % (m.built_for, fast_abi()))
         m.bind(check, {name: C.cast(getattr(L, name), C.c_void_p).value
                        for name in ("ugc_lookup_i64", "ugc_lookup_u32", "ugc_lookup_unique", "ugc_lookup_pool",
-                                    "ugc_record")})
+                                    "ugc_record", "ugc_route_plan_workspace", "ugc_route_plan", "ugc_route_dispatch",
+                                    "ugc_route_dispatch_grad", "ugc_route_combine", "ugc_route_combine_grad",
+                                    "ugc_adapter_add")})
         _fast = m
     return _fast
 

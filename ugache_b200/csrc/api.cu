@@ -29,6 +29,7 @@
 #include "device_types.h"
 #include "kernels.cuh"
 #include "placement.h"
+#include "routing.cuh"
 
 using namespace ugc;
 
@@ -2670,6 +2671,237 @@ int ugc_gen_table(void* dst, uint64_t seed, uint64_t row_begin, uint64_t n_rows,
   if (elem_bytes != 4 && elem_bytes != 2) return fail(UGC_ERR_INVALID, "elem_bytes must be 4 or 2");
   if (elem_bytes == 2 && dim % 2) return fail(UGC_ERR_INVALID, "fp16 rows need an even dim");
   UGC_CUDA(launch_gen_table(dst, seed, row_begin, n_rows, dim, elem_bytes, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+// -- routing ---------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// The calls without a context name their GPU: it is current inside the call, the caller's again behind it.
+struct OnDevice {
+  int before = -1;
+  bool changed = false;
+  int enter(int device) {
+    UGC_CUDA(cudaGetDevice(&before));
+    if (before == device) return UGC_OK;
+    UGC_CUDA(cudaSetDevice(device));
+    changed = true;
+    return UGC_OK;
+  }
+  ~OnDevice() {
+    if (changed) cudaSetDevice(before);
+  }
+};
+
+constexpr size_t kMaxRowDim = 1u << 28;
+
+int check_choices(size_t n_tokens, size_t k) {
+  if (k == 0) return fail(UGC_ERR_INVALID, "k must be at least 1");
+  if (n_tokens > kMaxBatch / k) return fail(UGC_ERR_INVALID, "%zu tokens of %zu choices: at most 2^28 choices per call", n_tokens, k);
+  return UGC_OK;
+}
+
+int elem_size(int elem_type) { return elem_type == UGC_ELEM_F32 ? 4 : 2; }
+
+// A matrix of n rows of dim elements; name for the message.
+int check_rows(const char* name, const void* p, int64_t stride, size_t dim, int elem_type) {
+  if (!p) return fail(UGC_ERR_INVALID, "%s must be non-null", name);
+  if (stride < 0 || (size_t)stride < dim || (size_t)stride > ((size_t)1 << 40))
+    return fail(UGC_ERR_INVALID, "%s: row stride %lld for rows of %zu elements", name, (long long)stride, dim);
+  if (reinterpret_cast<uintptr_t>(p) % elem_size(elem_type)) return fail(UGC_ERR_INVALID, "%s is not aligned to its elements", name);
+  return UGC_OK;
+}
+
+int check_words(const char* name, const void* p) {
+  if (!p) return fail(UGC_ERR_INVALID, "%s must be non-null", name);
+  if (reinterpret_cast<uintptr_t>(p) % 4) return fail(UGC_ERR_INVALID, "%s is not aligned to 4 bytes", name);
+  return UGC_OK;
+}
+
+// What the four calls that move rows have in common.
+int check_route(int elem_type, const float* weights, const int32_t* position, size_t n_tokens, size_t k, size_t dim) {
+  if (elem_type != UGC_ELEM_F32 && elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16)
+    return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
+  UGC_TRY(check_choices(n_tokens, k));
+  if (dim == 0 || dim > kMaxRowDim) return fail(UGC_ERR_INVALID, "rows of %zu elements: 1 to 2^28", dim);
+  if (n_tokens == 0) return UGC_OK;
+  if (n_tokens * dim > ((size_t)1 << 38)) return fail(UGC_ERR_INVALID, "%zu rows of %zu elements: at most 2^38 elements", n_tokens, dim);
+  UGC_TRY(check_words("position", position));
+  if (weights) UGC_TRY(check_words("weights", weights));
+  return UGC_OK;
+}
+
+RouteRows route_rows(const float* weights, const int32_t* position, size_t n_tokens, size_t k, size_t dim) {
+  RouteRows p{};
+  p.weights = weights;
+  p.position = position;
+  p.n_tokens = (uint32_t)n_tokens;
+  p.k = (uint32_t)k;
+  p.n_rows = (uint32_t)(n_tokens * k);
+  p.dim = (uint32_t)dim;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ugc_route_plan_workspace(size_t n_tokens, size_t k, int n_groups, size_t* bytes) {
+  if (!bytes) return fail(UGC_ERR_INVALID, "bytes must be non-null");
+  UGC_TRY(check_choices(n_tokens, k));
+  if (n_groups < 1 || n_groups > UGC_ROUTE_MAX_GROUPS)
+    return fail(UGC_ERR_INVALID, "%d groups: 1 to %d", n_groups, UGC_ROUTE_MAX_GROUPS);
+  *bytes = route_plan_scratch_bytes((uint32_t)(n_tokens * k), n_groups);
+  return UGC_OK;
+}
+
+int ugc_route_plan(int device_id, const void* ids, int id_bytes, size_t n_tokens, size_t k, int n_groups,
+                   int32_t* offsets, int32_t* order, int32_t* position, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  size_t need = 0;
+  UGC_TRY(ugc_route_plan_workspace(n_tokens, k, n_groups, &need));
+  if (id_bytes != 4 && id_bytes != 8) return fail(UGC_ERR_INVALID, "id_bytes must be 4 or 8");
+  UGC_TRY(check_words("offsets", offsets));
+  if (n_tokens) {
+    if (!ids || reinterpret_cast<uintptr_t>(ids) % id_bytes) return fail(UGC_ERR_INVALID, "ids must be non-null and aligned");
+    UGC_TRY(check_words("order", order));
+    UGC_TRY(check_words("position", position));
+  }
+  if (need) {
+    UGC_TRY(check_words("workspace", workspace));
+    if (workspace_bytes < need) return fail(UGC_ERR_INVALID, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  }
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_route_plan(ids, id_bytes, (uint32_t)(n_tokens * k), n_groups, offsets, order, position, workspace,
+                             static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_route_dispatch(int device_id, int elem_type, const void* x, int64_t x_stride, const float* weights,
+                       const int32_t* position, const int32_t* routed, size_t n_tokens, size_t k, size_t dim, void* out,
+                       int64_t out_stride, void* stream) {
+  UGC_TRY(check_route(elem_type, weights, position, n_tokens, k, dim));
+  if (n_tokens == 0) return UGC_OK;
+  UGC_TRY(check_rows("x", x, x_stride, dim, elem_type));
+  UGC_TRY(check_rows("out", out, out_stride, dim, elem_type));
+  if (routed) UGC_TRY(check_words("routed", routed));
+  RouteRows p = route_rows(weights, position, n_tokens, k, dim);
+  p.token_in = x, p.token_in_stride = x_stride * elem_size(elem_type);
+  p.row_out = out, p.row_out_stride = out_stride * elem_size(elem_type);
+  p.n_routed = routed;
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_route_spread(p, elem_type, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_route_dispatch_grad(int device_id, int elem_type, const void* dout, int64_t dout_stride, const void* x,
+                            int64_t x_stride, const float* weights, const int32_t* position, size_t n_tokens, size_t k,
+                            size_t dim, void* dx, int64_t dx_stride, float* dweights, void* stream) {
+  UGC_TRY(check_route(elem_type, weights, position, n_tokens, k, dim));
+  if (n_tokens == 0) return UGC_OK;
+  UGC_TRY(check_rows("dout", dout, dout_stride, dim, elem_type));
+  UGC_TRY(check_rows("dx", dx, dx_stride, dim, elem_type));
+  RouteRows p = route_rows(weights, position, n_tokens, k, dim);
+  if (dweights) {
+    UGC_TRY(check_rows("x", x, x_stride, dim, elem_type));
+    UGC_TRY(check_words("dweights", dweights));
+    p.token_in = x, p.token_in_stride = x_stride * elem_size(elem_type);
+    p.dots = dweights;
+  }
+  p.row_in = dout, p.row_in_stride = dout_stride * elem_size(elem_type);
+  p.token_out = dx, p.token_out_stride = dx_stride * elem_size(elem_type);
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_route_gather(p, elem_type, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_route_combine(int device_id, int elem_type, const void* rows, int64_t rows_stride, const float* weights,
+                      const int32_t* position, size_t n_tokens, size_t k, size_t dim, void* y, int64_t y_stride,
+                      void* stream) {
+  UGC_TRY(check_route(elem_type, weights, position, n_tokens, k, dim));
+  if (n_tokens == 0) return UGC_OK;
+  UGC_TRY(check_rows("rows", rows, rows_stride, dim, elem_type));
+  UGC_TRY(check_rows("y", y, y_stride, dim, elem_type));
+  RouteRows p = route_rows(weights, position, n_tokens, k, dim);
+  p.row_in = rows, p.row_in_stride = rows_stride * elem_size(elem_type);
+  p.token_out = y, p.token_out_stride = y_stride * elem_size(elem_type);
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_route_gather(p, elem_type, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t dy_stride, const void* rows,
+                           int64_t rows_stride, const float* weights, const int32_t* position, const int32_t* routed,
+                           size_t n_tokens, size_t k, size_t dim, void* drows, int64_t drows_stride, float* dweights,
+                           void* stream) {
+  UGC_TRY(check_route(elem_type, weights, position, n_tokens, k, dim));
+  if (n_tokens == 0) return UGC_OK;
+  UGC_TRY(check_rows("dy", dy, dy_stride, dim, elem_type));
+  UGC_TRY(check_rows("drows", drows, drows_stride, dim, elem_type));
+  if (routed) UGC_TRY(check_words("routed", routed));
+  RouteRows p = route_rows(weights, position, n_tokens, k, dim);
+  if (dweights) {
+    UGC_TRY(check_rows("rows", rows, rows_stride, dim, elem_type));
+    UGC_TRY(check_words("dweights", dweights));
+    p.row_in = rows, p.row_in_stride = rows_stride * elem_size(elem_type);
+    p.dots = dweights;
+  }
+  p.token_in = dy, p.token_in_stride = dy_stride * elem_size(elem_type);
+  p.row_out = drows, p.row_out_stride = drows_stride * elem_size(elem_type);
+  p.n_routed = routed;
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_route_spread(p, elem_type, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x, int64_t x_stride,
+                    const void* down, int64_t down_stride, const void* up, int64_t up_stride, const float* scale,
+                    const int32_t* offsets, const int32_t* order, size_t n_tokens, int n_groups, size_t rank, size_t dim,
+                    size_t out_dim, void* out, int64_t out_stride, void* stream) {
+  if (elem_type == UGC_ELEM_F32) return fail(UGC_ERR_UNSUPPORTED, "adapters are fp16 or bf16");
+  if (elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16) return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
+  UGC_TRY(check_choices(n_tokens, 1));
+  if (n_groups < 1 || n_groups > UGC_ROUTE_MAX_GROUPS)
+    return fail(UGC_ERR_INVALID, "%d groups: 1 to %d", n_groups, UGC_ROUTE_MAX_GROUPS);
+  if (rank == 0) return fail(UGC_ERR_INVALID, "rank must be at least 1");
+  if (rank > UGC_ADAPTER_MAX_RANK) return fail(UGC_ERR_UNSUPPORTED, "rank %zu: at most %d", rank, UGC_ADAPTER_MAX_RANK);
+  if (dim == 0 || dim > kMaxRowDim || out_dim == 0 || out_dim > kMaxRowDim)
+    return fail(UGC_ERR_INVALID, "%zu to %zu elements: 1 to 2^28", dim, out_dim);
+  if (n_tokens == 0) return UGC_OK;
+  UGC_TRY(check_rows("base", base, base_stride, out_dim, elem_type));
+  UGC_TRY(check_rows("out", out, out_stride, out_dim, elem_type));
+  UGC_TRY(check_rows("x", x, x_stride, dim, elem_type));
+  UGC_TRY(check_rows("down", down, down_stride, n_groups > 1 ? rank * dim : 0, elem_type));
+  UGC_TRY(check_rows("up", up, up_stride, n_groups > 1 ? rank * out_dim : 0, elem_type));
+  if (out == base && out_stride != base_stride) return fail(UGC_ERR_INVALID, "in place, out and base must have the same stride");
+  UGC_TRY(check_words("offsets", offsets));
+  UGC_TRY(check_words("order", order));
+  if (scale) UGC_TRY(check_words("scale", scale));
+  AdapterParams p{};
+  p.base = base, p.base_stride = base_stride;
+  p.x = x, p.x_stride = x_stride;
+  p.down = down, p.down_stride = down_stride;
+  p.up = up, p.up_stride = up_stride;
+  p.out = out, p.out_stride = out_stride;
+  p.scale = scale;
+  p.offsets = offsets;
+  p.order = order;
+  p.n_tokens = (uint32_t)n_tokens;
+  p.n_groups = (uint32_t)n_groups;
+  p.rank = (uint32_t)rank;
+  p.dim = (uint32_t)dim;
+  p.out_dim = (uint32_t)out_dim;
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(launch_adapter_add(p, elem_type, static_cast<cudaStream_t>(stream)));
   return UGC_OK;
 }
 

@@ -4,6 +4,7 @@ PyTorch appears here only to own device memory and streams; every operation is a
 into ``libugache_b200.so``, the per-step ones through the extension module ``_fast.so``.
 """
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 
@@ -346,6 +347,59 @@ class Cache:
                                          keys_u32.numel(), C.c_void_p(words.data_ptr()),
                                          C.c_void_p(s)))
         return words
+
+
+# -- routing: tokens grouped by the expert or adapter that serves them --------------------------
+class RoutePlan(NamedTuple):
+    """A batch of ids sorted by group, as ``route_plan`` makes it (all int32, on the GPU).
+
+    ``offsets[g]``: place where group ``g`` starts, ``n_groups + 1`` entries; ``order[p]``: flat index
+    (``t * k + j``) of the id at place ``p``, the ids outside the groups last; ``position``: place of every
+    id, in the shape of the ids, -1 outside the groups."""
+    offsets: "torch.Tensor"   # noqa: F821
+    order: "torch.Tensor"     # noqa: F821
+    position: "torch.Tensor"  # noqa: F821
+
+
+def route_plan(ids, n_groups, stream=None):
+    """Sorts the ids of a batch into ``n_groups`` groups (stable, on the GPU; nothing synchronises).
+    ids: CUDA int64 / int32 tensor, ``[T]`` or ``[T, k]`` with ``k`` choices a token; an id outside
+    ``[0, n_groups)`` is a dropped choice.  The plan serves every layer that uses the same ids."""
+    return RoutePlan(*(_lib._fast or _lib.fast()).route_plan(ids, n_groups, stream))
+
+
+def route_dispatch(x, plan, weights=None, out=None, stream=None):
+    """``out[position[t, j]] = weights[t, j] * x[t]``: rows of tokens ``[T, dim]`` to their groups' order
+    ``[T * k, dim]`` (copied without weights).  Rows behind the last group, which no choice takes, are
+    zero.  Rows are float32, float16 or bfloat16, weights float32."""
+    return (_lib._fast or _lib.fast()).route_dispatch(x, plan.offsets, plan.position, weights, out, stream)
+
+
+def route_dispatch_grad(dout, plan, weights=None, x=None, dx=None, stream=None):
+    """Gradients of ``route_dispatch``: ``(dx, dweights)``; ``dweights`` is None unless ``x`` is given."""
+    return (_lib._fast or _lib.fast()).route_dispatch_grad(dout, plan.offsets, plan.position, weights, x, dx, stream)
+
+
+def route_combine(rows, plan, weights=None, out=None, stream=None):
+    """``out[t] = sum over j of weights[t, j] * rows[position[t, j]]``: rows in the groups' order back to
+    their tokens, ``[T, dim]``; summed in fp32 in the order of the choices, rounded once.  Dropped choices
+    add nothing."""
+    return (_lib._fast or _lib.fast()).route_combine(rows, plan.offsets, plan.position, weights, out, stream)
+
+
+def route_combine_grad(dy, plan, weights=None, rows=None, drows=None, stream=None):
+    """Gradients of ``route_combine``: ``(drows, dweights)``; ``dweights`` is None unless ``rows`` is given.
+    Rows of ``drows`` behind the last group are zero."""
+    return (_lib._fast or _lib.fast()).route_combine_grad(dy, plan.offsets, plan.position, weights, rows, drows, stream)
+
+
+def adapter_add(base, x, down, up, plan, scale=None, out=None, stream=None):
+    """``out[t] = base[t] + scale[a] * (x[t] @ down[a].T) @ up[a].T`` with ``a`` the adapter of token ``t`` in
+    ``plan`` (one id a token); tokens without one: ``base[t]``.  base ``[T, out_dim]`` (what the shared projection gave),
+    x ``[T, dim]``, down ``[adapters, rank, dim]``, up ``[adapters, out_dim, rank]``: float16 or bfloat16; scale
+    float32 ``[adapters]``.  ``out`` may be ``base``.  Adapters kept as rows of a cache: ``down`` and ``up`` are views of the
+    rows of ``Cache.lookup_unique`` and its ``inverse`` the ids of the plan."""
+    return (_lib._fast or _lib.fast()).adapter_add(base, x, down, up, plan.offsets, plan.order, scale, out, stream)
 
 
 def gen_table(dst_ptr, seed, row_begin, n_rows, dim, elem_bytes, stream=0):
