@@ -479,13 +479,19 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
  * out may be base itself (same stride); other overlaps are not allowed.  fp16 and bf16, rank at most
  * UGC_ADAPTER_MAX_RANK; 16-byte aligned addresses and strides, dims and ranks in multiples of 8
  * elements take the fast loads.  Sums are fp32; the rank products enter the second product as two
- * 16-bit terms (16 significand bits or more). */
+ * 16-bit terms (16 significand bits or more).  workspace: ugc_adapter_workspace bytes (0 for small
+ * batches, then NULL will do), 16-byte aligned, free again when the call's work is done. */
 #define UGC_ADAPTER_MAX_RANK 128
+int ugc_adapter_workspace(size_t n_tokens, int n_groups, size_t rank, size_t dim, size_t out_dim, size_t* bytes);
 int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x,
                     int64_t x_stride, const void* down, int64_t down_stride, const void* up, int64_t up_stride,
                     const float* scale, const int32_t* offsets, const int32_t* order, size_t n_tokens,
                     int n_groups, size_t rank, size_t dim, size_t out_dim, void* out, int64_t out_stride,
-                    void* stream);
+                    void* workspace, size_t workspace_bytes, void* stream);
+/* The prompt kernels wait for their own copies and products; a wait that does not end within about two
+ * seconds ends the kernel (its outputs are then unfinished) and is counted per GPU.  Reads that count,
+ * synchronising; 0 on a sound machine. */
+int ugc_adapter_stalled(int device_id, uint32_t* count);
 
 /* -- introspection --------------------------------------------------------------------- */
 int ugc_stats(ugc_ctx* ctx, int replica_id, ugc_stats_t* out);

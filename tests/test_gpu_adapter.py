@@ -68,8 +68,9 @@ class Case:
 
 @pytest.mark.parametrize("elem", sorted(TYPES))
 @pytest.mark.parametrize("rank", [1, 4, 8, 12, 16, 24, 32, 40, 64, 72, 128])
-def test_ranks(rt, rank, elem):
-    Case(rt, 77, 5, rank, 512, 320, elem).check(rt)
+@pytest.mark.parametrize("T", [77, 1000])   # single tokens, prompts
+def test_ranks(rt, rank, elem, T):
+    Case(rt, T, 5, rank, 512, 320, elem).check(rt)
 
 
 @pytest.mark.parametrize("dim,out_dim", [(1, 1), (8, 8), (33, 17), (256, 256), (264, 1000), (1001, 77), (4096, 40), (72, 4096), (2048, 2056)])
@@ -86,27 +87,29 @@ def test_tokens(rt, T, G):
 
 @pytest.mark.parametrize("rank", [16, 64])
 @pytest.mark.parametrize("what", ["one adapter", "own adapters", "none", "ragged", "no one without"])
-def test_groupings(rt, what, rank):
-    T, G = 520, 1024
+@pytest.mark.parametrize("G", [32, 1024])   # prompts, single tokens
+def test_groupings(rt, what, rank, G):
+    T = 520
     i = torch.arange(T, device="cuda")
-    ids = {"one adapter": torch.full_like(i, 1023), "own adapters": i, "none": torch.full_like(i, -1),
-           "ragged": (i.float().sqrt() * 2).long(), "no one without": i % 3}[what]
+    ids = {"one adapter": torch.full_like(i, G - 1), "own adapters": i % G, "none": torch.full_like(i, -1),
+           "ragged": (i.float().sqrt() * 1.3).long(), "no one without": i % 3}[what]
     c = Case(rt, T, G, rank, 256, 128, "f16", ids=ids)
     c.check(rt)
 
 
 @pytest.mark.parametrize("elem", sorted(TYPES))
-def test_in_place_and_strided(rt, elem):
-    c = Case(rt, 150, 4, 16, 256, 192, elem)
+@pytest.mark.parametrize("T", [150, 600])
+def test_in_place_and_strided(rt, elem, T):
+    c = Case(rt, T, 4, 16, 256, 192, elem)
     want, slack = formula(c.base, c.x, c.down, c.up, c.ids, c.scale)
     base = c.base.clone()
     got = rt.adapter_add(base, c.x, c.down, c.up, c.plan, scale=c.scale, out=base)
     assert got.data_ptr() == base.data_ptr() and bool(((base.double() - want).abs() <= slack).all())
     for pad in (8, 1):     # on and off the 16-byte boundaries
-        wide = torch.full((150, 192 + 2 * pad), 3.0, dtype=c.base.dtype, device="cuda")
+        wide = torch.full((T, 192 + 2 * pad), 3.0, dtype=c.base.dtype, device="cuda")
         view = wide[:, pad:pad + 192]
         view.copy_(c.base)
-        x = torch.zeros((150, 256 + pad), dtype=c.base.dtype, device="cuda")[:, :256]
+        x = torch.zeros((T, 256 + pad), dtype=c.base.dtype, device="cuda")[:, :256]
         x.copy_(c.x)
         rt.adapter_add(view, x, c.down, c.up, c.plan, scale=c.scale, out=view)
         assert bool(((view.double() - want).abs() <= slack).all())
@@ -114,10 +117,11 @@ def test_in_place_and_strided(rt, elem):
         assert bool((wide == 3.0).all())
 
 
-def test_both_matrices_in_one_row(rt):
+@pytest.mark.parametrize("T", [90, 2000])
+def test_both_matrices_in_one_row(rt, T):
     """An adapter as a row of a table: down and up behind one another."""
     G, r, H, N = 7, 16, 320, 256
-    c = Case(rt, 90, G, r, H, N, "bf16")
+    c = Case(rt, T, G, r, H, N, "bf16")
     table = torch.cat([c.down.reshape(G, -1), c.up.reshape(G, -1)], 1)
     want = rt.adapter_add(c.base, c.x, c.down, c.up, c.plan, scale=c.scale)
     c.down, c.up = table[:, :r * H].view(G, r, H), table[:, r * H:].view(G, N, r)
@@ -126,43 +130,48 @@ def test_both_matrices_in_one_row(rt):
 
 
 @pytest.mark.parametrize("elem", sorted(TYPES))
-def test_magnitudes(rt, elem):
+@pytest.mark.parametrize("T", [60, 800])
+def test_magnitudes(rt, elem, T):
     """Rank products far above and below the type's range; the result is in it."""
     for factor in (2.0 ** 17, 2.0 ** -20):
-        c = Case(rt, 60, 3, 16, 256, 128, elem, scaled=False)
+        c = Case(rt, T, 3, 16, 256, 128, elem, scaled=False)
         c.scale = torch.full((3,), factor, device="cuda")
         c.up = (c.up.float() * (2.0 ** -14 if factor > 1 else 1)).to(c.up.dtype)
         c.check(rt)
 
 
-def test_non_finite_values_stay_with_their_token(rt):
-    c = Case(rt, 64, 3, 16, 256, 128, "bf16", none=0.0)
+@pytest.mark.parametrize("T", [64, 900])
+def test_non_finite_values_stay_with_their_token(rt, T):
+    c = Case(rt, T, 3, 16, 256, 128, "bf16", none=0.0)
     clean = rt.adapter_add(c.base, c.x, c.down, c.up, c.plan)
     c.x[5, 3], c.x[6, 7] = float("nan"), float("inf")
     got = rt.adapter_add(c.base, c.x, c.down, c.up, c.plan)
-    rest = torch.arange(64, device="cuda")
+    rest = torch.arange(T, device="cuda")
     rest = rest[(rest != 5) & (rest != 6)]
     assert torch.equal(got[rest], clean[rest])
     assert bool(torch.isnan(got[5]).all()) and not bool(torch.isfinite(got[6]).any())
 
 
-def test_adapters_that_no_token_names_are_not_read(rt):
-    c = Case(rt, 64, 4, 16, 256, 128, "bf16")
+@pytest.mark.parametrize("T", [64, 900])
+def test_adapters_that_no_token_names_are_not_read(rt, T):
+    c = Case(rt, T, 4, 16, 256, 128, "bf16")
     c.ids = torch.where(c.ids == 2, torch.full_like(c.ids, 1), c.ids)
     c.plan = rt.route_plan(c.ids, 4)
     c.down[2], c.up[2] = float("nan"), float("nan")
     c.check(rt)
 
 
-def test_token_results_do_not_depend_on_the_batch(rt):
-    c = Case(rt, 300, 5, 16, 512, 256, "bf16", none=0.0)
+@pytest.mark.parametrize("T", [300, 5000])
+def test_same_results_again(rt, T):
+    c = Case(rt, T, 5, 16, 512, 256, "bf16", none=0.0)
     whole = rt.adapter_add(c.base, c.x, c.down, c.up, c.plan, scale=c.scale)
     assert torch.equal(whole, rt.adapter_add(c.base, c.x, c.down, c.up, c.plan, scale=c.scale))
 
 
-def test_far_adapters(rt):
-    """Adapter and row offsets beyond 32 bits."""
-    c = Case(rt, 40, 3, 8, 64, 64, "f16")
+@pytest.mark.parametrize("T", [40, 700])
+def test_far_adapters(rt, T):
+    """Adapter offsets beyond 32 bits."""
+    c = Case(rt, T, 3, 8, 64, 64, "f16")
     stride = (1 << 30) + 64
     room = torch.empty(3 * stride, dtype=torch.float16, device="cuda")
     down, up = room.as_strided((3, 8, 64), (stride, 64, 1)), room.as_strided((3, 64, 8), (stride, 8, 1), 1024)
@@ -170,6 +179,32 @@ def test_far_adapters(rt):
     up.copy_(c.up)
     c.down, c.up = down, up
     c.check(rt)
+
+
+@pytest.mark.parametrize("elem", sorted(TYPES))
+def test_far_rows(rt, elem):
+    """Row offsets beyond 32 bits, in elements and in bytes; prompts."""
+    c = Case(rt, 520, 2, 16, 64, 64, elem)
+    stride = (1 << 23) + 8           # 520 rows of it pass 2^32 elements
+    room = torch.empty(520 * stride, dtype=c.base.dtype, device="cuda")
+    base, x = room.as_strided((520, 64), (stride, 1)), room.as_strided((520, 64), (stride, 1), 1024)
+    base.copy_(c.base)
+    x.copy_(c.x)
+    want, slack = formula(c.base, c.x, c.down, c.up, c.ids, c.scale)
+    rt.adapter_add(base, x, c.down, c.up, c.plan, scale=c.scale, out=base)
+    assert bool(((base.double() - want).abs() <= slack).all())
+    few = rt.route_plan(c.ids[-20:], 2)                        # single tokens: the last rows of the room
+    got = rt.adapter_add(c.base[-20:], x[-20:], c.down, c.up, few, scale=c.scale)
+    assert bool(((got.double() - want[-20:]).abs() <= slack[-20:]).all())
+
+
+def test_no_wait_ran_out(rt):
+    import ctypes as C
+
+    from ugache_b200 import _lib
+    n = C.c_uint32(7)
+    _lib.check(_lib.lib().ugc_adapter_stalled(0, C.byref(n)))
+    assert n.value == 0
 
 
 def test_refusals(rt):
@@ -189,8 +224,9 @@ def test_refusals(rt):
             call()
 
 
-def test_captured_and_replayed(rt):
-    c = Case(rt, 64, 9, 16, 512, 256, "bf16")
+@pytest.mark.parametrize("T", [64, 3000])
+def test_captured_and_replayed(rt, T):
+    c = Case(rt, T, 9, 16, 512, 256, "bf16")
     out = torch.empty_like(c.base)
 
     def step():
@@ -202,7 +238,7 @@ def test_captured_and_replayed(rt):
     with torch.cuda.graph(g):
         step()
     for i in range(3):
-        c.ids.copy_(torch.randint(-1, 9, (64,), device="cuda"))
+        c.ids.copy_(torch.randint(-1, 9, (T,), device="cuda"))
         c.x.normal_()
         g.replay()
         want, slack = formula(c.base, c.x, c.down, c.up, c.ids, c.scale)

@@ -67,9 +67,10 @@ def test_no_tokens(L, call):
 
 
 def adapter(L, elem=2, base=A, base_stride=8, x=A, x_stride=16, down=A, down_stride=64, up=A, up_stride=64, scale=None, offsets=D,
-            order=D, tokens=4, groups=3, rank=4, dim=16, out_dim=8, out=B, out_stride=8):
+            order=D, tokens=4, groups=3, rank=4, dim=16, out_dim=8, out=B, out_stride=8,
+            space=None, size=0):
     return L.ugc_adapter_add(0, elem, base, base_stride, x, x_stride, down, down_stride, up, up_stride, scale, offsets, order,
-                             tokens, groups, rank, dim, out_dim, out, out_stride, None)
+                             tokens, groups, rank, dim, out_dim, out, out_stride, space, size, None)
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -78,10 +79,19 @@ def adapter(L, elem=2, base=A, base_stride=8, x=A, x_stride=16, down=A, down_str
     (dict(tokens=(1 << 28) + 1), INVALID), (dict(base=None), INVALID), (dict(x=A + 1), INVALID), (dict(x_stride=15), INVALID),
     (dict(base_stride=7), INVALID), (dict(out=None), INVALID), (dict(down=None), INVALID), (dict(down_stride=63), INVALID),
     (dict(up_stride=31), INVALID), (dict(offsets=None), INVALID), (dict(order=None), INVALID), (dict(scale=D + 2), INVALID),
-    (dict(out=A, out_stride=16), INVALID)])
+    (dict(out=A, out_stride=16), INVALID), (dict(tokens=8192), INVALID), (dict(tokens=8192, space=A, size=1 << 10), INVALID),
+    (dict(tokens=8192, space=A + 8, size=1 << 30), INVALID)])
 def test_adapter(L, kw, status):
     assert adapter(L, **kw) == status
     assert L.ugc_last_error()
+
+
+def test_adapter_workspace(L):
+    n = C.c_size_t(1)
+    assert L.ugc_adapter_workspace(4, 3, 4, 16, 8, C.byref(n)) == 0 and n.value == 0
+    assert L.ugc_adapter_workspace(8192, 3, 4, 16, 8, C.byref(n)) == 0 and n.value > 0
+    assert L.ugc_adapter_workspace(8192, 3, 4, 16, 8, None) == INVALID
+    assert L.ugc_adapter_stalled(0, None) == INVALID
 
 
 def test_adapter_no_tokens(L):

@@ -184,8 +184,10 @@ SIGNATURES = {
     "ugc_route_dispatch_grad": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P, _P]),
     "ugc_route_combine": (_I, [_I, _I, _P, _I64, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P]),
     "ugc_route_combine_grad": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _P, _P, _SZ, _SZ, _SZ, _P, _I64, _P, _P]),
+    "ugc_adapter_workspace": (_I, [_SZ, _I, _SZ, _SZ, _SZ, C.POINTER(_SZ)]),
     "ugc_adapter_add": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _SZ, _I, _SZ, _SZ, _SZ, _P,
-                             _I64, _P]),
+                             _I64, _P, _SZ, _P]),
+    "ugc_adapter_stalled": (_I, [_I, C.POINTER(C.c_uint32)]),
     "ugc_stats": (_I, [_P, _I, C.POINTER(Stats)]),
     "ugc_get_tuning": (_I, [_P, _I, C.POINTER(Tuning)]),
     "ugc_set_tuning": (_I, [_P, _I, C.POINTER(Tuning)]),
@@ -257,7 +259,7 @@ def fast():
                        for name in ("ugc_lookup_i64", "ugc_lookup_u32", "ugc_lookup_unique", "ugc_lookup_pool",
                                     "ugc_record", "ugc_route_plan_workspace", "ugc_route_plan", "ugc_route_dispatch",
                                     "ugc_route_dispatch_grad", "ugc_route_combine", "ugc_route_combine_grad",
-                                    "ugc_adapter_add")})
+                                    "ugc_adapter_workspace", "ugc_adapter_add")})
         _fast = m
     return _fast
 

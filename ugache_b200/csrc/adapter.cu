@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -76,19 +77,20 @@ __device__ __forceinline__ float unit_scale(float max) {
   return max > 0.f && e > -120 && e < 126 ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
 }
 
-// The tile of this cluster: tiles of 16 tokens, group by group, those without a group last.
+// Tile `index` of the batch: tiles of ROWS tokens, group by group, those without a group last.  By the whole CTA.
 struct Tile {
   uint32_t group, first, count;  // first: place in `order`
 };
+template <int ROWS, int THREADS>
 __device__ Tile find_tile(const int32_t* offsets, uint32_t n_groups, uint32_t n_tokens, uint32_t index) {
-  __shared__ uint32_t partial[kWarps];
+  __shared__ uint32_t partial[THREADS / 32];
   __shared__ Tile found;
-  const uint32_t n = n_groups + 1, per = (n + kBlock - 1) / kBlock, g0 = threadIdx.x * per;
+  const uint32_t n = n_groups + 1, per = (n + THREADS - 1) / THREADS, g0 = threadIdx.x * per;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto begin_of = [&](uint32_t g) { return min((uint32_t)max(offsets[g], 0), n_tokens); };
   auto tiles_of = [&](uint32_t g) {
     const uint32_t a = begin_of(g), b = g < n_groups ? begin_of(g + 1) : n_tokens;
-    return b > a ? (b - a + kTile - 1) / kTile : 0;
+    return b > a ? (b - a + ROWS - 1) / ROWS : 0;
   };
   uint32_t sum = 0;
   for (uint32_t i = 0; i < per; i++)
@@ -109,8 +111,8 @@ __device__ Tile find_tile(const int32_t* offsets, uint32_t n_groups, uint32_t n_
       const uint32_t m = tiles_of(g0 + i);
       if (index < at + m) {
         const uint32_t a = begin_of(g0 + i), b = g0 + i < n_groups ? begin_of(g0 + i + 1) : n_tokens;
-        const uint32_t first = a + (index - at) * kTile;
-        found = Tile{g0 + i, first, min(b - first, (uint32_t)kTile)};
+        const uint32_t first = a + (index - at) * ROWS;
+        found = Tile{g0 + i, first, min(b - first, (uint32_t)ROWS)};
         break;
       }
       at += m;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p) {
   __shared__ int32_t token[kTile];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t member = cluster.block_rank();
-  const Tile tile = find_tile(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / kCluster);
+  const Tile tile = find_tile<kTile, kBlock>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / kCluster);
   if (tile.count == 0) return;  // of the whole cluster
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   if (threadIdx.x < kTile) {
@@ -293,6 +295,448 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p) {
   }
 }
 
+// ------------------------------------------------------------------------------------
+// prompts: tiles of 128 tokens on the 5th-generation tensor cores
+// ------------------------------------------------------------------------------------
+// Two launches.  The first multiplies a tile's rows of x with the adapter's `down`, every CTA a slice of dim,
+// and leaves fp32 partial sums in the workspace; the second adds those up, splits them into two
+// 16-bit terms and multiplies them with `up`, every CTA a slice of out_dim, adding `base` on the way out.
+// Both stream 64 columns a step through a ring of stages in shared memory: four warps copy
+// (token rows lie anywhere, so 16 bytes a thread), one thread issues the matrix instructions, four
+// warps take the products out of tensor memory.
+//
+// Operands lie in shared memory as 8-row blocks of 16 bytes a row (128 bytes), the blocks of a column
+// of 16 bytes behind one another: a quarter warp copies one block, and one token a thread reads a column
+// of `base`, both without bank conflicts.
+
+constexpr int kBigTile = 128;
+constexpr int kStep = 64;                                   // columns a step
+constexpr int kRowsBytes = kBigTile * kStep * 2;            // x or base of a step
+constexpr int kProducers = 128;
+constexpr int kDownThreads = kProducers + 32;
+constexpr int kUpThreads = kProducers + 128 + 32;
+
+__device__ unsigned int g_stalled;  // waits that ran out
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// False after about two seconds: nothing here takes that long, so something is broken and the kernel ends.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+  long long began = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    const long long now = clock64();
+    if (!began) began = now;
+    if (now - began > 4000000000ll) {
+      atomicAdd(&g_stalled, 1u);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_left() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void order_for_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Operand in shared memory, without swizzle: `column` bytes from one 16-byte column to the next, 128 from 8 rows to the next.
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t column) {
+  return (uint64_t)(address >> 4 & 0x3fff) | (uint64_t)(column >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | 1ull << 46;
+}
+// 128 x n products of 16-bit values, both operands with their depth contiguous, fp32 sums.
+template <typename E>
+__host__ __device__ constexpr uint32_t instruction(int n) {
+  const uint32_t type = std::is_same<E, __half>::value ? 0 : 1;
+  return 1u << 4 | type << 7 | type << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(kBigTile >> 4) << 24;
+}
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(what), "r"(add ? 1u : 0u)
+      : "memory");
+}
+// The barrier gets an arrival when the matrix instructions issued so far are done.
+__device__ __forceinline__ void arrive_behind_products(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tensor_memory(uint32_t* slot) {  // by one warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(slot)), "n"(COLUMNS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void free_tensor_memory(uint32_t at) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(COLUMNS));
+}
+// 16 columns of the warp's 32 lanes, one lane a thread.
+__device__ __forceinline__ void from_tensor_memory(float (&v)[16], uint32_t at) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// A producer thread's share of a step's token rows: rows 8 * (warp + 4 * i) + lane % 8, 16-byte columns
+// lane / 8 and lane / 8 + 4; eight neighbouring threads write one 128-byte block.
+struct RowCopies {
+  const uint16_t* row[4];  // nullptr: no token there
+  __device__ void set(const void* rows, long long stride, const int32_t* token) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int t = token[8 * (warp + 4 * i) + (lane & 7)];
+      row[i] = t < 0 ? nullptr : static_cast<const uint16_t*>(rows) + (long long)t * stride;
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t to, uint32_t column, uint32_t end) const {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t c = (lane >> 3) + 4 * h, at = column + c * 8;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (row[i]) copy16(to + c * (kBigTile * 16) + (8 * (warp + 4 * i) + (lane & 7)) * 16, at < end ? row[i] + at : row[i], at < end);
+    }
+  }
+};
+
+// n_rows x (8 * n_columns) elements of a matrix into blocks; rows from live_rows on and columns from live_end on are zeros.
+template <int N_ROWS, int N_COLUMNS>
+__device__ __forceinline__ void copy_matrix(uint32_t to, const uint16_t* from, size_t stride, uint32_t row, uint32_t live_rows,
+                                            uint32_t column, uint32_t live_end) {
+  static_assert(N_ROWS * N_COLUMNS % kProducers == 0, "every thread copies the same number");
+#pragma unroll
+  for (int i = 0; i < N_ROWS * N_COLUMNS / kProducers; i++) {
+    const uint32_t item = threadIdx.x + i * kProducers, c = item / 8 % N_COLUMNS, r = item / (8 * N_COLUMNS) * 8 + item % 8;
+    const uint32_t at = column + c * 8;
+    const bool live = row + r < live_rows && at < live_end;
+    copy16(to + c * (N_ROWS * 16) + r * 16, live ? from + (row + r) * stride + at : from, live);
+  }
+}
+
+template <int RP>
+struct BigShape {
+  static constexpr int kMatrixBytes = RP * kStep * 2;              // down or up of a step
+  static constexpr int kStageBytes = kRowsBytes + kMatrixBytes;
+  static constexpr int kTermBytes = kBigTile * RP * 2;             // the rank products, one term
+  // two CTAs an SM up to rank 64; one above
+  static constexpr int kDownStages = 4;
+  static constexpr int kUpStages = RP <= 64 ? 3 : 4;
+  static constexpr int kDownShared = kDownStages * kStageBytes + 1024;
+  static constexpr int kUpShared = kUpStages * kStageBytes + 2 * kTermBytes + 1024;
+};
+
+__device__ __forceinline__ uint32_t aligned_shared(unsigned char* smem) { return (shared_address(smem) + 1023) / 1024 * 1024; }
+
+// inner[split][place][RP] = x rows of the tile times a slice of `down`
+template <typename E, int RP>
+__global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, uint32_t splits) {
+  using S = BigShape<RP>;
+  constexpr int kStages = S::kDownStages, kLag = kStages - 1, kColumns = RP < 32 ? 32 : RP;
+  extern __shared__ unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int32_t token[kBigTile];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Tile tile = find_tile<kBigTile, kDownThreads>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / splits);
+  if (tile.count == 0 || tile.group == p.n_groups) return;
+  const uint32_t split = blockIdx.x % splits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t steps_all = (p.dim + kStep - 1) / kStep;
+  const uint32_t step0 = (uint32_t)((unsigned long long)steps_all * split / splits);
+  const uint32_t steps = (uint32_t)((unsigned long long)steps_all * (split + 1) / splits) - step0;  // at least one: splits <= steps_all
+  if (threadIdx.x < kBigTile) {
+    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
+    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      barrier_init(shared_address(&full[i]), kProducers);
+      barrier_init(shared_address(&empty[i]), 1);
+    }
+    barrier_init(shared_address(&done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) tensor_memory<kColumns>(&tmem_slot);
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem);
+
+  if (warp < 4) {
+    RowCopies x;
+    x.set(p.x, p.x_stride, token);
+    const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
+    bool ok = true;
+    for (uint32_t i = 0; ok && i < steps + kLag; i++) {
+      const uint32_t s = i % kStages;
+      if (i < steps) {
+        if (i >= kStages) ok = barrier_wait(shared_address(&empty[s]), (i / kStages - 1) & 1);
+        if (!ok) break;
+        const uint32_t to = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
+        x.issue(to, column, p.dim);
+        copy_matrix<RP, 8>(to + kRowsBytes, down, p.dim, 0, p.rank, column, p.dim);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i >= kLag) {
+        copies_left<kLag>();
+        order_for_tensor_cores();
+        barrier_arrive(shared_address(&full[(i - kLag) % kStages]));
+      }
+    }
+    copies_left<0>();
+    // the tile's products: one token a thread
+    if (ok && barrier_wait(shared_address(&done), 0)) {
+      after_sync();
+      float* to = inner + ((size_t)split * p.n_tokens + tile.first + threadIdx.x) * RP;
+#pragma unroll
+      for (int c = 0; c < RP; c += 16) {
+        float v[16];
+        from_tensor_memory(v, tmem + (warp * 32 << 16) + c);
+        loads_done();
+        if (threadIdx.x < tile.count) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+      }
+    }
+  } else if (lane == 0) {
+    bool ok = true;
+    for (uint32_t i = 0; i < steps; i++) {
+      const uint32_t s = i % kStages;
+      ok = barrier_wait(shared_address(&full[s]), i / kStages & 1);
+      if (!ok) break;
+      after_sync();
+      const uint32_t at = ring + s * S::kStageBytes;
+#pragma unroll
+      for (int k = 0; k < kStep / 16; k++)
+        multiply(tmem, operand(at + k * 2 * kBigTile * 16, kBigTile * 16), operand(at + kRowsBytes + k * 2 * RP * 16, RP * 16),
+                 instruction<E>(RP), i > 0 || k > 0);
+      arrive_behind_products(shared_address(&empty[s]));
+    }
+    if (ok) arrive_behind_products(shared_address(&done));
+  }
+  before_sync();
+  __syncthreads();
+  after_sync();
+  if (warp == 4) free_tensor_memory<kColumns>(tmem);
+}
+
+template <typename E, int RP>
+__global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
+    adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, uint32_t splits, uint32_t slices) {
+  using S = BigShape<RP>;
+  constexpr int kStages = S::kUpStages, kLag = kStages - 1, kColumns = 2 * kStep;
+  extern __shared__ unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kStages], drained[kStages], product[2], taken[2], terms;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int32_t token[kBigTile];
+  // the launch ahead (the first product) started behind everything that wrote base, up and the plan
+  const Tile tile = find_tile<kBigTile, kUpThreads>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / slices);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool copy_only = tile.group == p.n_groups;
+  if (tile.count == 0 || (copy_only && p.out == p.base)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const uint32_t slice = blockIdx.x % slices;
+  const uint32_t steps_all = (p.out_dim + kStep - 1) / kStep;
+  const uint32_t step0 = (uint32_t)((unsigned long long)steps_all * slice / slices);
+  const uint32_t steps = (uint32_t)((unsigned long long)steps_all * (slice + 1) / slices) - step0;
+  if (threadIdx.x < kBigTile) {
+    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
+    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
+  }
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+  if (copy_only) {
+    __syncthreads();
+    const uint16_t* base = static_cast<const uint16_t*>(p.base);
+    const uint32_t begin = step0 * kStep, end = min(p.out_dim, begin + steps * kStep);
+    for (uint32_t m = warp; m < tile.count; m += kUpThreads / 32) {
+      if (token[m] < 0) continue;
+      for (uint32_t n = begin + lane * 8; n < end; n += 256)
+        *reinterpret_cast<uint4*>(out + (long long)token[m] * p.out_stride + n) =
+            *reinterpret_cast<const uint4*>(base + (long long)token[m] * p.base_stride + n);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      barrier_init(shared_address(&full[i]), kProducers);
+      barrier_init(shared_address(&drained[i]), 4);
+    }
+    for (int i = 0; i < 2; i++) {
+      barrier_init(shared_address(&product[i]), 1);
+      barrier_init(shared_address(&taken[i]), 4);
+    }
+    barrier_init(shared_address(&terms), 128);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tensor_memory<kColumns>(&tmem_slot);
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem), term = ring + kStages * S::kStageBytes;
+
+  if (warp < 4) {
+    RowCopies base;
+    base.set(p.base, p.base_stride, token);
+    const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
+    for (uint32_t i = 0; i < steps + kLag; i++) {
+      const uint32_t s = i % kStages;
+      if (i < steps) {
+        if (i >= kStages && !barrier_wait(shared_address(&drained[s]), (i / kStages - 1) & 1)) break;
+        const uint32_t to = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
+        base.issue(to, column, p.out_dim);
+        copy_matrix<kStep, RP / 8>(to + kRowsBytes, up, p.rank, column, p.out_dim, 0, p.rank);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i >= kLag) {
+        copies_left<kLag>();
+        order_for_tensor_cores();
+        barrier_arrive(shared_address(&full[(i - kLag) % kStages]));
+      }
+    }
+    copies_left<0>();
+  } else if (warp < 8) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t row = threadIdx.x - kProducers, quarter = warp - 4;
+    float back;
+    {  // the token's rank products: added up, scaled so that the largest is in [1, 2), in two terms
+      const float scale = p.scale ? p.scale[tile.group] : 1.f;
+      const float* from = inner + ((size_t)tile.first + min(row, tile.count - 1)) * RP;
+      float u[RP], top = 0.f;
+#pragma unroll
+      for (int c = 0; c < RP; c += 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c));
+        u[c] = v.x, u[c + 1] = v.y, u[c + 2] = v.z, u[c + 3] = v.w;
+      }
+      for (uint32_t m = 1; m < splits; m++) {
+        from += (size_t)p.n_tokens * RP;
+#pragma unroll
+        for (int c = 0; c < RP; c += 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c));
+          u[c] += v.x, u[c + 1] += v.y, u[c + 2] += v.z, u[c + 3] += v.w;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < RP; c++) {
+        u[c] *= scale;
+        top = fmaxf(top, fabsf(u[c]));
+      }
+      const float s = unit_scale(top);
+      back = 1.f / s;
+#pragma unroll
+      for (int c = 0; c < RP; c += 8) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float a = u[c + 2 * i] * s, b = u[c + 2 * i + 1] * s;
+          hi[i] = Half<E>::narrow(a, b);
+          const float2 h = Half<E>::widen(hi[i]);
+          lo[i] = Half<E>::narrow(isinf(h.x) ? 0.f : a - h.x, isinf(h.y) ? 0.f : b - h.y);
+        }
+        const uint32_t at = term + (c / 8) * (kBigTile * 16) + row * 16;
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + S::kTermBytes), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+      }
+    }
+    order_for_tensor_cores();
+    barrier_arrive(shared_address(&terms));
+    uint16_t* to[4];  // where the thread's rows of the way out go, as in RowCopies
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int t = token[quarter * 32 + 8 * i + (lane & 7)];
+      to[i] = t < 0 ? nullptr : out + (long long)t * p.out_stride;
+    }
+    for (uint32_t i = 0; i < steps; i++) {
+      const uint32_t s = i % kStages, at = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
+      if (!barrier_wait(shared_address(&full[s]), i / kStages & 1) || !barrier_wait(shared_address(&product[i & 1]), i / 2 & 1)) break;
+      after_sync();
+#pragma unroll
+      for (int c = 0; c < kStep; c += 16) {
+        float v[16];
+        from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + c);
+        loads_done();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t piece = at + (c / 8 + h) * (kBigTile * 16) + row * 16;
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece) : "memory");
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float2 b = Half<E>::widen(w[j]);
+            w[j] = Half<E>::narrow(fmaf(v[8 * h + 2 * j], back, b.x), fmaf(v[8 * h + 2 * j + 1], back, b.y));
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(piece), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+      }
+      before_sync();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t c = (lane >> 3) + 4 * h;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(at + c * (kBigTile * 16) + (quarter * 32 + 8 * j + (lane & 7)) * 16)
+                       : "memory");
+          if (to[j] && column + c * 8 < p.out_dim) *reinterpret_cast<uint4*>(to[j] + column + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_address(&drained[s]));
+    }
+  } else if (lane == 0) {
+    bool ok = barrier_wait(shared_address(&terms), 0);
+    for (uint32_t i = 0; ok && i < steps; i++) {
+      const uint32_t s = i % kStages, at = ring + s * S::kStageBytes + kRowsBytes;
+      ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) &&
+           (i < 2 || barrier_wait(shared_address(&taken[i & 1]), (i / 2 - 1) & 1));
+      if (!ok) break;
+      after_sync();
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int k = 0; k < RP / 16; k++)
+          multiply(tmem + (i & 1) * kStep, operand(term + t * S::kTermBytes + k * 2 * kBigTile * 16, kBigTile * 16),
+                   operand(at + k * 2 * kStep * 16, kStep * 16), instruction<E>(kStep), t > 0 || k > 0);
+      arrive_behind_products(shared_address(&product[i & 1]));
+    }
+  }
+  before_sync();
+  __syncthreads();
+  after_sync();
+  if (warp == 8) free_tensor_memory<kColumns>(tmem);
+}
+
 template <typename E, int RP>
 cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t stream) {
   auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
@@ -317,9 +761,60 @@ cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t str
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+// How a batch of prompts is split: CTAs a tile of the first and of the second product.
+struct BigSplit {
+  uint32_t tiles, splits, slices;
+};
+BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t dim, uint32_t out_dim) {
+  constexpr uint32_t kSlots = 2 * 148;
+  BigSplit b;
+  b.tiles = n_tokens / kBigTile + std::min(n_groups + 1, n_tokens);  // at most: every group may end in a tile of its own
+  const uint32_t k = (dim + kStep - 1) / kStep, n = (out_dim + kStep - 1) / kStep;
+  b.splits = std::min({(kSlots + b.tiles - 1) / b.tiles, k, 8u});
+  b.slices = std::min((2 * kSlots + b.tiles - 1) / b.tiles, n);
+  return b;
+}
+int padded_rank(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+
+bool big_batch(uint32_t n_tokens, uint32_t n_groups) { return n_tokens >= 512 && n_tokens >= 16 * n_groups; }
+
+template <typename E, int RP>
+cudaError_t big_launch(const AdapterParams& p, float* inner, cudaStream_t stream) {
+  using S = BigShape<RP>;
+  auto down = adapter_down_kernel<E, RP>;
+  auto up = adapter_up_kernel<E, RP>;
+  cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kDownShared);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kUpShared);
+  if (e != cudaSuccess) return e;
+  const BigSplit b = big_split(p.n_tokens, p.n_groups, p.dim, p.out_dim);
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(b.tiles * b.splits);
+  cfg.blockDim = dim3(kDownThreads);
+  cfg.dynamicSmemBytes = S::kDownShared;
+  e = cudaLaunchKernelEx(&cfg, down, p, inner, b.splits);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(b.tiles * b.slices);
+  cfg.blockDim = dim3(kUpThreads);
+  cfg.dynamicSmemBytes = S::kUpShared;
+  return cudaLaunchKernelEx(&cfg, up, p, static_cast<const float*>(inner), b.splits, b.slices);
+}
+
 }  // namespace
 
-cudaError_t launch_adapter_add(const AdapterParams& p, int elem, cudaStream_t stream) {
+size_t adapter_scratch_bytes(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t dim, uint32_t out_dim) {
+  if (!big_batch(n_tokens, n_groups)) return 0;
+  return (size_t)big_split(n_tokens, n_groups, dim, out_dim).splits * n_tokens * padded_rank(rank) * sizeof(float);
+}
+
+cudaError_t adapter_stalled(uint32_t* count) { return cudaMemcpyFromSymbol(count, g_stalled, sizeof(*count)); }
+
+cudaError_t launch_adapter_add(const AdapterParams& p, int elem, void* scratch, cudaStream_t stream) {
   if (p.n_tokens == 0) return cudaSuccess;
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(p.base) | reinterpret_cast<uintptr_t>(p.x) |
                               reinterpret_cast<uintptr_t>(p.down) | reinterpret_cast<uintptr_t>(p.up) |
@@ -328,6 +823,15 @@ cudaError_t launch_adapter_add(const AdapterParams& p, int elem, cudaStream_t st
   const bool vector = addresses % 16 == 0 && strides % 8 == 0 && p.dim % 8 == 0 && p.out_dim % 8 == 0 && p.rank % 8 == 0;
   auto by_rank = [&](auto e) {
     using E = decltype(e);
+    if (vector && big_batch(p.n_tokens, p.n_groups)) {
+      float* inner = static_cast<float*>(scratch);
+      switch (padded_rank(p.rank)) {
+        case 16: return big_launch<E, 16>(p, inner, stream);
+        case 32: return big_launch<E, 32>(p, inner, stream);
+        case 64: return big_launch<E, 64>(p, inner, stream);
+        default: return big_launch<E, 128>(p, inner, stream);
+      }
+    }
     if (p.rank <= 8) return adapter_launch<E, 8>(p, vector, stream);
     if (p.rank <= 16) return adapter_launch<E, 16>(p, vector, stream);
     if (p.rank <= 32) return adapter_launch<E, 32>(p, vector, stream);

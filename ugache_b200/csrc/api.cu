@@ -2862,12 +2862,8 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
   return UGC_OK;
 }
 
-int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x, int64_t x_stride,
-                    const void* down, int64_t down_stride, const void* up, int64_t up_stride, const float* scale,
-                    const int32_t* offsets, const int32_t* order, size_t n_tokens, int n_groups, size_t rank, size_t dim,
-                    size_t out_dim, void* out, int64_t out_stride, void* stream) {
-  if (elem_type == UGC_ELEM_F32) return fail(UGC_ERR_UNSUPPORTED, "adapters are fp16 or bf16");
-  if (elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16) return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
+int ugc_adapter_workspace(size_t n_tokens, int n_groups, size_t rank, size_t dim, size_t out_dim, size_t* bytes) {
+  if (!bytes) return fail(UGC_ERR_INVALID, "bytes must be non-null");
   UGC_TRY(check_choices(n_tokens, 1));
   if (n_groups < 1 || n_groups > UGC_ROUTE_MAX_GROUPS)
     return fail(UGC_ERR_INVALID, "%d groups: 1 to %d", n_groups, UGC_ROUTE_MAX_GROUPS);
@@ -2875,6 +2871,18 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
   if (rank > UGC_ADAPTER_MAX_RANK) return fail(UGC_ERR_UNSUPPORTED, "rank %zu: at most %d", rank, UGC_ADAPTER_MAX_RANK);
   if (dim == 0 || dim > kMaxRowDim || out_dim == 0 || out_dim > kMaxRowDim)
     return fail(UGC_ERR_INVALID, "%zu to %zu elements: 1 to 2^28", dim, out_dim);
+  *bytes = adapter_scratch_bytes((uint32_t)n_tokens, (uint32_t)n_groups, (uint32_t)rank, (uint32_t)dim, (uint32_t)out_dim);
+  return UGC_OK;
+}
+
+int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x, int64_t x_stride,
+                    const void* down, int64_t down_stride, const void* up, int64_t up_stride, const float* scale,
+                    const int32_t* offsets, const int32_t* order, size_t n_tokens, int n_groups, size_t rank, size_t dim,
+                    size_t out_dim, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  UGC_TRY(ugc_adapter_workspace(n_tokens, n_groups, rank, dim, out_dim, &need));
+  if (elem_type == UGC_ELEM_F32) return fail(UGC_ERR_UNSUPPORTED, "adapters are fp16 or bf16");
+  if (elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16) return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
   if (n_tokens == 0) return UGC_OK;
   UGC_TRY(check_rows("base", base, base_stride, out_dim, elem_type));
   UGC_TRY(check_rows("out", out, out_stride, out_dim, elem_type));
@@ -2885,6 +2893,10 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
   UGC_TRY(check_words("offsets", offsets));
   UGC_TRY(check_words("order", order));
   if (scale) UGC_TRY(check_words("scale", scale));
+  if (need) {
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return fail(UGC_ERR_INVALID, "workspace must be non-null and 16-byte aligned");
+    if (workspace_bytes < need) return fail(UGC_ERR_INVALID, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  }
   AdapterParams p{};
   p.base = base, p.base_stride = base_stride;
   p.x = x, p.x_stride = x_stride;
@@ -2901,7 +2913,15 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
   p.out_dim = (uint32_t)out_dim;
   OnDevice on;
   UGC_TRY(on.enter(device_id));
-  UGC_CUDA(launch_adapter_add(p, elem_type, static_cast<cudaStream_t>(stream)));
+  UGC_CUDA(launch_adapter_add(p, elem_type, workspace, static_cast<cudaStream_t>(stream)));
+  return UGC_OK;
+}
+
+int ugc_adapter_stalled(int device_id, uint32_t* count) {
+  if (!count) return fail(UGC_ERR_INVALID, "count must be non-null");
+  OnDevice on;
+  UGC_TRY(on.enter(device_id));
+  UGC_CUDA(adapter_stalled(count));
   return UGC_OK;
 }
 

@@ -31,6 +31,7 @@ struct Entry {
   decltype(&ugc_route_dispatch_grad) route_dispatch_grad;
   decltype(&ugc_route_combine) route_combine;
   decltype(&ugc_route_combine_grad) route_combine_grad;
+  decltype(&ugc_adapter_workspace) adapter_workspace;
   decltype(&ugc_adapter_add) adapter_add;
 };
 Entry g_ugc = {};
@@ -549,17 +550,23 @@ PyObject* fast_adapter_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       (a[6] != Py_None && !words_arg(a[6], "scale", &c, at::kFloat, groups, &scale)) ||
       (a[7] != Py_None && !rows_arg(a[7], "out", &c, tokens, false, out_dim, true, &out)))
     return nullptr;
+  const int n_groups = (int)std::min(groups, (int64_t)1 << 30);
+  size_t bytes = 0;
+  int rc = g_ugc.adapter_workspace((size_t)tokens, n_groups, (size_t)rank, (size_t)dim, (size_t)out_dim, &bytes);
+  if (rc != UGC_OK) return raise_status(rc);
+  at::Tensor space;
+  if (bytes) space = device_empty({(int64_t)bytes}, at::kByte, c.dev);
+  void* wp = bytes ? space.data_ptr() : nullptr;
   if (!out.defined()) out = device_empty({tokens, out_dim}, c.ty, c.dev);
   const void *bp = base.data_ptr(), *xp = x.data_ptr(), *dp = down.data_ptr(), *upp = up.data_ptr();
   const float* sp = scale.defined() ? scale.data_ptr<float>() : nullptr;
   const int32_t *fp = offsets.data_ptr<int32_t>(), *rp = order.data_ptr<int32_t>();
   void* op = out.data_ptr();
   const int64_t ds = groups > 1 ? down.stride(0) : rank * dim, us = groups > 1 ? up.stride(0) : rank * out_dim;
-  int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = g_ugc.adapter_add(c.dev.index(), elem_type(c), bp, row_stride(base), xp, row_stride(x), dp, ds, upp, us, sp, fp, rp,
-                         (size_t)tokens, (int)std::min(groups, (int64_t)1 << 30), (size_t)rank, (size_t)dim, (size_t)out_dim,
-                         op, row_stride(out), on.stream);
+                         (size_t)tokens, n_groups, (size_t)rank, (size_t)dim, (size_t)out_dim,
+                         op, row_stride(out), wp, bytes, on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
   return THPVariable_Wrap(std::move(out));
@@ -582,7 +589,8 @@ PyObject* fast_bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       !address("ugc_route_plan", &g_ugc.route_plan) || !address("ugc_route_dispatch", &g_ugc.route_dispatch) ||
       !address("ugc_route_dispatch_grad", &g_ugc.route_dispatch_grad) ||
       !address("ugc_route_combine", &g_ugc.route_combine) ||
-      !address("ugc_route_combine_grad", &g_ugc.route_combine_grad) || !address("ugc_adapter_add", &g_ugc.adapter_add))
+      !address("ugc_route_combine_grad", &g_ugc.route_combine_grad) ||
+      !address("ugc_adapter_workspace", &g_ugc.adapter_workspace) || !address("ugc_adapter_add", &g_ugc.adapter_add))
     return nullptr;
   Py_XDECREF(g_check);
   g_check = Py_NewRef(a[0]);

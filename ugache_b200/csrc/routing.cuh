@@ -50,6 +50,9 @@ struct AdapterParams {
   long long base_stride, x_stride, down_stride, up_stride, out_stride;
   uint32_t n_tokens, n_groups, rank, dim, out_dim;
 };
-cudaError_t launch_adapter_add(const AdapterParams& p, int elem, cudaStream_t stream);
+// scratch: adapter_scratch_bytes, 16-byte aligned
+size_t adapter_scratch_bytes(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t dim, uint32_t out_dim);
+cudaError_t launch_adapter_add(const AdapterParams& p, int elem, void* scratch, cudaStream_t stream);
+cudaError_t adapter_stalled(uint32_t* count);
 
 }  // namespace ugc
