@@ -298,23 +298,28 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p) {
 // ------------------------------------------------------------------------------------
 // prompts: tiles of 128 tokens on the 5th-generation tensor cores
 // ------------------------------------------------------------------------------------
-// Two launches.  The first multiplies a tile's rows of x with the adapter's `down`, every CTA a slice of dim,
-// and leaves fp32 partial sums in the workspace; the second adds those up, splits them into two
-// 16-bit terms and multiplies them with `up`, every CTA a slice of out_dim, adding `base` on the way out.
-// Both stream 64 columns a step through a ring of stages in shared memory: four warps copy
-// (token rows lie anywhere, so 16 bytes a thread), one thread issues the matrix instructions, four
-// warps take the products out of tensor memory.
+// Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
+// partial sums in the workspace; the second adds those up, splits them into two 16-bit terms and multiplies
+// them with `up`, adding `base` on the way out.  In both a tile is so many steps of 64 columns, the tiles of the
+// batch stand one behind the other, and every CTA of a full GPU takes the same number of consecutive
+// steps, so that no number of tiles leaves part of the GPU idle; where a CTA's run starts or ends inside a tile
+// of the first product, the tile has one more partial sum.
+// Steps go through a ring of stages in shared memory: four warps copy (token rows lie anywhere, so 16
+// bytes a thread), one thread issues the matrix instructions, the other warps take the products out of
+// tensor memory.
 //
-// Operands lie in shared memory as 8-row blocks of 16 bytes a row (128 bytes), the blocks of a column
-// of 16 bytes behind one another: a quarter warp copies one block, and one token a thread reads a column
-// of `base`, both without bank conflicts.
+// Operands lie in shared memory in rows of 128 bytes whose 16-byte pieces are exchanged by row (piece c
+// of row r at c ^ (r % 8)), as the matrix unit reads them: a line of global memory is a line there, and
+// one token a thread reads `base` without bank conflicts.  (Blocks of 8 rows x 16 bytes, the other layout
+// the unit takes, split every line over eight and cost 2.5 times the time.)
 
 constexpr int kBigTile = 128;
 constexpr int kStep = 64;                                   // columns a step
 constexpr int kRowsBytes = kBigTile * kStep * 2;            // x or base of a step
 constexpr int kProducers = 128;
-constexpr int kDownThreads = kProducers + 32;
-constexpr int kUpThreads = kProducers + 128 + 32;
+constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, multiply
+constexpr int kUpThreads = kProducers + 256 + 32;
+constexpr int kMostTiles = 36;                              // a CTA's run touches
 
 __device__ unsigned int g_stalled;  // waits that ran out
 
@@ -349,16 +354,18 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void copies_left() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// What the thread has written or been told of becomes visible to the matrix instructions issued behind it.
+// For copied operands the issuing thread does this, behind the barrier: a copying thread's fence would wait
+// for its copies of later steps too.
 __device__ __forceinline__ void order_for_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Operand in shared memory, without swizzle: `column` bytes from one 16-byte column to the next, 128 from 8 rows to the next.
-__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t column) {
-  return (uint64_t)(address >> 4 & 0x3fff) | (uint64_t)(column >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | 1ull << 46;
+// Operand in shared memory: rows of 128 bytes with exchanged pieces, 1024 bytes from 8 rows to the next.
+__device__ __forceinline__ uint64_t operand(uint32_t address) {
+  return (uint64_t)(address >> 4 & 0x3fff) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
+// 16-byte piece c of row r
+__device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 // 128 x n products of 16-bit values, both operands with their depth contiguous, fp32 sums.
 template <typename E>
 __host__ __device__ constexpr uint32_t instruction(int n) {
@@ -399,342 +406,442 @@ __device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A producer thread's share of a step's token rows: rows 8 * (warp + 4 * i) + lane % 8, 16-byte columns
-// lane / 8 and lane / 8 + 4; eight neighbouring threads write one 128-byte block.
+__device__ __forceinline__ int token_at(const AdapterParams& p, const Tile& tile, uint32_t place) {
+  const uint32_t t = place < tile.count ? (uint32_t)p.order[tile.first + place] : kFull;
+  return t < p.n_tokens ? (int)t : -1;
+}
+
+// The barrier gets the thread's arrival when the copies that it has issued so far have landed.
+__device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// A thread's share of a step's token rows, one of four warps: piece lane % 8 of rows 4 * (warp + 4 * i) + lane / 8.
 struct RowCopies {
-  const uint16_t* row[4];  // nullptr: no token there
-  __device__ void set(const void* rows, long long stride, const int32_t* token) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint16_t* row[8];  // nullptr: no token there
+  __device__ __forceinline__ void set(const void* rows, long long stride, const AdapterParams& p, const Tile& tile) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int t = token[8 * (warp + 4 * i) + (lane & 7)];
-      row[i] = t < 0 ? nullptr : static_cast<const uint16_t*>(rows) + (long long)t * stride;
+    for (int i = 0; i < 8; i++) {
+      const int t = token_at(p, tile, place(i));
+      row[i] = t < 0 ? nullptr : static_cast<const uint16_t*>(rows) + (long long)t * stride + (threadIdx.x & 7) * 8;
     }
   }
+  static __device__ __forceinline__ uint32_t place(int i) { return 4 * ((threadIdx.x >> 5) + 4 * i) + (threadIdx.x >> 3 & 3); }
   __device__ __forceinline__ void issue(uint32_t to, uint32_t column, uint32_t end) const {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool live = column + (threadIdx.x & 7) * 8 < end;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t c = (lane >> 3) + 4 * h, at = column + c * 8;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (row[i]) copy16(to + c * (kBigTile * 16) + (8 * (warp + 4 * i) + (lane & 7)) * 16, at < end ? row[i] + at : row[i], at < end);
-    }
+    for (int i = 0; i < 8; i++)
+      if (row[i]) copy16(to + piece_at(place(i), threadIdx.x & 7), live ? row[i] + column : row[i], live);
   }
 };
 
-// n_rows x (8 * n_columns) elements of a matrix into blocks; rows from live_rows on and columns from live_end on are zeros.
-template <int N_ROWS, int N_COLUMNS>
+// N_ROWS x (8 * N_PIECES) elements of a matrix; beyond 64 elements a row goes on in another block of all rows.
+// Rows from live_rows on and columns from live_end on are zeros.
+template <int N_ROWS, int N_PIECES>
 __device__ __forceinline__ void copy_matrix(uint32_t to, const uint16_t* from, size_t stride, uint32_t row, uint32_t live_rows,
                                             uint32_t column, uint32_t live_end) {
-  static_assert(N_ROWS * N_COLUMNS % kProducers == 0, "every thread copies the same number");
+  static_assert(N_ROWS * N_PIECES % kProducers == 0, "every thread copies the same number");
 #pragma unroll
-  for (int i = 0; i < N_ROWS * N_COLUMNS / kProducers; i++) {
-    const uint32_t item = threadIdx.x + i * kProducers, c = item / 8 % N_COLUMNS, r = item / (8 * N_COLUMNS) * 8 + item % 8;
-    const uint32_t at = column + c * 8;
+  for (int i = 0; i < N_ROWS * N_PIECES / kProducers; i++) {
+    const uint32_t item = threadIdx.x + i * kProducers, c = item % N_PIECES, r = item / N_PIECES, at = column + c * 8;
     const bool live = row + r < live_rows && at < live_end;
-    copy16(to + c * (N_ROWS * 16) + r * 16, live ? from + (row + r) * stride + at : from, live);
+    copy16(to + c / 8 * (N_ROWS * 128) + piece_at(r, c % 8), live ? from + (row + r) * stride + at : from, live);
   }
 }
 
 template <int RP>
 struct BigShape {
-  static constexpr int kMatrixBytes = RP * kStep * 2;              // down or up of a step
-  static constexpr int kStageBytes = kRowsBytes + kMatrixBytes;
-  static constexpr int kTermBytes = kBigTile * RP * 2;             // the rank products, one term
+  static constexpr int kDownStage = kRowsBytes + RP * 128;                      // x, down
+  static constexpr int kUpStage = kRowsBytes + (RP + 63) / 64 * kStep * 128;    // base, up
+  static constexpr int kTermBytes = (2 * RP + 63) / 64 * kBigTile * 128;        // the rank products: first terms, then second
   // two CTAs an SM up to rank 64; one above
   static constexpr int kDownStages = 4;
   static constexpr int kUpStages = RP <= 64 ? 3 : 4;
-  static constexpr int kDownShared = kDownStages * kStageBytes + 1024;
-  static constexpr int kUpShared = kUpStages * kStageBytes + 2 * kTermBytes + 1024;
+  static constexpr int kDownShared = kDownStages * kDownStage + 1024;
+  static constexpr int kUpShared = kUpStages * kUpStage + kTermBytes + 1024;
 };
 
 __device__ __forceinline__ uint32_t aligned_shared(unsigned char* smem) { return (shared_address(smem) + 1023) / 1024 * 1024; }
 
-// inner[split][place][RP] = x rows of the tile times a slice of `down`
+// How many steps a CTA of a launch takes.
+struct BigShare {
+  uint32_t tile_steps;  // steps of a tile
+  uint32_t least;       // steps of a run, at least
+  uint32_t grid;
+  __device__ __forceinline__ uint32_t run(uint32_t tiles) const {
+    return max((uint32_t)(((unsigned long long)tiles * tile_steps + grid - 1) / grid), least);
+  }
+};
+
+// A CTA's run: its tiles and the steps of each.
+struct Run {
+  uint32_t tiles;          // tiles with an adapter in the batch
+  uint32_t first, count;   // tiles of the run
+  unsigned long long begin, end;
+  uint32_t tile_steps;
+  __device__ __forceinline__ uint32_t from(uint32_t i) const {
+    const unsigned long long at = (unsigned long long)(first + i) * tile_steps;
+    return begin > at ? (uint32_t)(begin - at) : 0;
+  }
+  __device__ __forceinline__ uint32_t to(uint32_t i) const {
+    const unsigned long long at = (unsigned long long)(first + i) * tile_steps;
+    return (uint32_t)min(end - at, (unsigned long long)tile_steps);
+  }
+};
+
+// By the whole CTA; `bare`: tiles of tokens without an adapter count as well.
+template <int THREADS>
+__device__ Run find_run(const AdapterParams& p, const BigShare& share, bool bare, Tile* found) {
+  __shared__ uint32_t partial[THREADS / 32], total[2];
+  const uint32_t n = p.n_groups + 1, per = (n + THREADS - 1) / THREADS, g0 = threadIdx.x * per;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto begin_of = [&](uint32_t g) { return min((uint32_t)max(p.offsets[g], 0), p.n_tokens); };
+  auto tile_of = [&](uint32_t g) {  // the group as one tile
+    const uint32_t a = begin_of(g), b = g < p.n_groups ? begin_of(g + 1) : p.n_tokens;
+    return Tile{g, a, b > a ? b - a : 0};
+  };
+  uint32_t sum = 0;
+  for (uint32_t i = 0; i < per; i++)
+    if (g0 + i < n) sum += (tile_of(g0 + i).count + kBigTile - 1) / kBigTile;
+  uint32_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(kFull, inc, d);
+    if (lane >= d) inc += o;
+  }
+  if (lane == 31) partial[warp] = inc;
+  __syncthreads();
+  uint32_t at = inc - sum;
+  for (uint32_t w = 0; w < warp; w++) at += partial[w];
+  for (uint32_t i = 0, t = at; i < per && g0 + i < n; i++) {
+    if (g0 + i == p.n_groups) total[0] = t;
+    t += (tile_of(g0 + i).count + kBigTile - 1) / kBigTile;
+    if (g0 + i == p.n_groups) total[1] = t;
+  }
+  __syncthreads();
+  Run r;
+  r.tiles = total[0];
+  r.tile_steps = share.tile_steps;
+  const uint32_t all = bare ? total[1] : total[0];
+  const unsigned long long steps = share.run(all);
+  r.begin = min(blockIdx.x * steps, (unsigned long long)all * share.tile_steps);
+  r.end = min(r.begin + steps, (unsigned long long)all * share.tile_steps);
+  r.first = (uint32_t)(r.begin / share.tile_steps);
+  r.count = r.end > r.begin ? min((uint32_t)((r.end - 1) / share.tile_steps) - r.first + 1, (uint32_t)kMostTiles) : 0;
+  if (at < r.first + r.count && at + sum > r.first) {
+    for (uint32_t i = 0; i < per && g0 + i < n; i++) {
+      const Tile g = tile_of(g0 + i);
+      for (uint32_t o = 0; o < g.count; o += kBigTile, at++)
+        if (at >= r.first && at < r.first + r.count) found[at - r.first] = Tile{g.group, g.first + o, min(g.count - o, (uint32_t)kBigTile)};
+    }
+  }
+  __syncthreads();
+  return r;
+}
+
+// inner[part] = x rows of the tile times a run of columns of `down`; a tile's RP products a token lie as
+// [RP / 4][tokens][4], so that one token a thread writes and reads whole lines.
 template <typename E, int RP>
-__global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, uint32_t splits) {
+__global__ void __launch_bounds__(kDownThreads, RP <= 64 ? 2 : 1) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, BigShare share) {
   using S = BigShape<RP>;
-  constexpr int kStages = S::kDownStages, kLag = kStages - 1, kColumns = RP < 32 ? 32 : RP;
+  constexpr int kStages = S::kDownStages, kColumns = 2 * RP;
   extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], ready[2], taken[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int32_t token[kBigTile];
+  __shared__ Tile tiles[kMostTiles];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Tile tile = find_tile<kBigTile, kDownThreads>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / splits);
-  if (tile.count == 0 || tile.group == p.n_groups) return;
-  const uint32_t split = blockIdx.x % splits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t steps_all = (p.dim + kStep - 1) / kStep;
-  const uint32_t step0 = (uint32_t)((unsigned long long)steps_all * split / splits);
-  const uint32_t steps = (uint32_t)((unsigned long long)steps_all * (split + 1) / splits) - step0;  // at least one: splits <= steps_all
-  if (threadIdx.x < kBigTile) {
-    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
-    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
-  }
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Run run = find_run<kDownThreads>(p, share, false, tiles);
+  if (run.count == 0) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; i++) {
       barrier_init(shared_address(&full[i]), kProducers);
       barrier_init(shared_address(&empty[i]), 1);
     }
-    barrier_init(shared_address(&done), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 4) tensor_memory<kColumns>(&tmem_slot);
-  before_sync();
-  __syncthreads();
-  after_sync();
-  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem);
-
-  if (warp < 4) {
-    RowCopies x;
-    x.set(p.x, p.x_stride, token);
-    const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
-    bool ok = true;
-    for (uint32_t i = 0; ok && i < steps + kLag; i++) {
-      const uint32_t s = i % kStages;
-      if (i < steps) {
-        if (i >= kStages) ok = barrier_wait(shared_address(&empty[s]), (i / kStages - 1) & 1);
-        if (!ok) break;
-        const uint32_t to = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
-        x.issue(to, column, p.dim);
-        copy_matrix<RP, 8>(to + kRowsBytes, down, p.dim, 0, p.rank, column, p.dim);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (i >= kLag) {
-        copies_left<kLag>();
-        order_for_tensor_cores();
-        barrier_arrive(shared_address(&full[(i - kLag) % kStages]));
-      }
-    }
-    copies_left<0>();
-    // the tile's products: one token a thread
-    if (ok && barrier_wait(shared_address(&done), 0)) {
-      after_sync();
-      float* to = inner + ((size_t)split * p.n_tokens + tile.first + threadIdx.x) * RP;
-#pragma unroll
-      for (int c = 0; c < RP; c += 16) {
-        float v[16];
-        from_tensor_memory(v, tmem + (warp * 32 << 16) + c);
-        loads_done();
-        if (threadIdx.x < tile.count) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
-      }
-    }
-  } else if (lane == 0) {
-    bool ok = true;
-    for (uint32_t i = 0; i < steps; i++) {
-      const uint32_t s = i % kStages;
-      ok = barrier_wait(shared_address(&full[s]), i / kStages & 1);
-      if (!ok) break;
-      after_sync();
-      const uint32_t at = ring + s * S::kStageBytes;
-#pragma unroll
-      for (int k = 0; k < kStep / 16; k++)
-        multiply(tmem, operand(at + k * 2 * kBigTile * 16, kBigTile * 16), operand(at + kRowsBytes + k * 2 * RP * 16, RP * 16),
-                 instruction<E>(RP), i > 0 || k > 0);
-      arrive_behind_products(shared_address(&empty[s]));
-    }
-    if (ok) arrive_behind_products(shared_address(&done));
-  }
-  before_sync();
-  __syncthreads();
-  after_sync();
-  if (warp == 4) free_tensor_memory<kColumns>(tmem);
-}
-
-template <typename E, int RP>
-__global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
-    adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, uint32_t splits, uint32_t slices) {
-  using S = BigShape<RP>;
-  constexpr int kStages = S::kUpStages, kLag = kStages - 1, kColumns = 2 * kStep;
-  extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kStages], drained[kStages], product[2], taken[2], terms;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int32_t token[kBigTile];
-  // the launch ahead (the first product) started behind everything that wrote base, up and the plan
-  const Tile tile = find_tile<kBigTile, kUpThreads>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / slices);
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool copy_only = tile.group == p.n_groups;
-  if (tile.count == 0 || (copy_only && p.out == p.base)) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const uint32_t slice = blockIdx.x % slices;
-  const uint32_t steps_all = (p.out_dim + kStep - 1) / kStep;
-  const uint32_t step0 = (uint32_t)((unsigned long long)steps_all * slice / slices);
-  const uint32_t steps = (uint32_t)((unsigned long long)steps_all * (slice + 1) / slices) - step0;
-  if (threadIdx.x < kBigTile) {
-    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
-    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
-  }
-  uint16_t* out = static_cast<uint16_t*>(p.out);
-  if (copy_only) {
-    __syncthreads();
-    const uint16_t* base = static_cast<const uint16_t*>(p.base);
-    const uint32_t begin = step0 * kStep, end = min(p.out_dim, begin + steps * kStep);
-    for (uint32_t m = warp; m < tile.count; m += kUpThreads / 32) {
-      if (token[m] < 0) continue;
-      for (uint32_t n = begin + lane * 8; n < end; n += 256)
-        *reinterpret_cast<uint4*>(out + (long long)token[m] * p.out_stride + n) =
-            *reinterpret_cast<const uint4*>(base + (long long)token[m] * p.base_stride + n);
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; i++) {
-      barrier_init(shared_address(&full[i]), kProducers);
-      barrier_init(shared_address(&drained[i]), 4);
-    }
     for (int i = 0; i < 2; i++) {
-      barrier_init(shared_address(&product[i]), 1);
+      barrier_init(shared_address(&ready[i]), 1);
       barrier_init(shared_address(&taken[i]), 4);
     }
-    barrier_init(shared_address(&terms), 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) tensor_memory<kColumns>(&tmem_slot);
   before_sync();
   __syncthreads();
   after_sync();
-  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem), term = ring + kStages * S::kStageBytes;
+  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem);
 
   if (warp < 4) {
-    RowCopies base;
-    base.set(p.base, p.base_stride, token);
-    const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
-    for (uint32_t i = 0; i < steps + kLag; i++) {
-      const uint32_t s = i % kStages;
-      if (i < steps) {
-        if (i >= kStages && !barrier_wait(shared_address(&drained[s]), (i / kStages - 1) & 1)) break;
-        const uint32_t to = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
-        base.issue(to, column, p.out_dim);
-        copy_matrix<kStep, RP / 8>(to + kRowsBytes, up, p.rank, column, p.out_dim, 0, p.rank);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (i >= kLag) {
-        copies_left<kLag>();
-        order_for_tensor_cores();
-        barrier_arrive(shared_address(&full[(i - kLag) % kStages]));
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
+      const Tile tile = tiles[n];
+      RowCopies x;
+      x.set(p.x, p.x_stride, p, tile);
+      const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        const uint32_t s = i % kStages;
+        if (i >= kStages && !(ok = barrier_wait(shared_address(&empty[s]), (i / kStages - 1) & 1))) break;
+        const uint32_t to = ring + s * S::kDownStage, column = k * kStep;
+        x.issue(to, column, p.dim);
+        copy_matrix<RP, 8>(to + kRowsBytes, down, p.dim, 0, p.rank, column, p.dim);
+        arrive_behind_copies(shared_address(&full[s]));
       }
     }
-    copies_left<0>();
+    copies_done();
   } else if (warp < 8) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t row = threadIdx.x - kProducers, quarter = warp - 4;
-    float back;
-    {  // the token's rank products: added up, scaled so that the largest is in [1, 2), in two terms
-      const float scale = p.scale ? p.scale[tile.group] : 1.f;
-      const float* from = inner + ((size_t)tile.first + min(row, tile.count - 1)) * RP;
-      float u[RP], top = 0.f;
-#pragma unroll
-      for (int c = 0; c < RP; c += 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c));
-        u[c] = v.x, u[c + 1] = v.y, u[c + 2] = v.z, u[c + 3] = v.w;
-      }
-      for (uint32_t m = 1; m < splits; m++) {
-        from += (size_t)p.n_tokens * RP;
-#pragma unroll
-        for (int c = 0; c < RP; c += 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c));
-          u[c] += v.x, u[c + 1] += v.y, u[c + 2] += v.z, u[c + 3] += v.w;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < RP; c++) {
-        u[c] *= scale;
-        top = fmaxf(top, fabsf(u[c]));
-      }
-      const float s = unit_scale(top);
-      back = 1.f / s;
-#pragma unroll
-      for (int c = 0; c < RP; c += 8) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float a = u[c + 2 * i] * s, b = u[c + 2 * i + 1] * s;
-          hi[i] = Half<E>::narrow(a, b);
-          const float2 h = Half<E>::widen(hi[i]);
-          lo[i] = Half<E>::narrow(isinf(h.x) ? 0.f : a - h.x, isinf(h.y) ? 0.f : b - h.y);
-        }
-        const uint32_t at = term + (c / 8) * (kBigTile * 16) + row * 16;
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + S::kTermBytes), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
-      }
-    }
-    order_for_tensor_cores();
-    barrier_arrive(shared_address(&terms));
-    uint16_t* to[4];  // where the thread's rows of the way out go, as in RowCopies
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int t = token[quarter * 32 + 8 * i + (lane & 7)];
-      to[i] = t < 0 ? nullptr : out + (long long)t * p.out_stride;
-    }
-    for (uint32_t i = 0; i < steps; i++) {
-      const uint32_t s = i % kStages, at = ring + s * S::kStageBytes, column = (step0 + i) * kStep;
-      if (!barrier_wait(shared_address(&full[s]), i / kStages & 1) || !barrier_wait(shared_address(&product[i & 1]), i / 2 & 1)) break;
+    const uint32_t row = threadIdx.x - kProducers;
+    for (uint32_t n = 0; n < run.count; n++) {
+      const Tile tile = tiles[n];
+      if (!barrier_wait(shared_address(&ready[n & 1]), n / 2 & 1)) break;
       after_sync();
+      const uint32_t part = blockIdx.x - (uint32_t)((unsigned long long)(run.first + n) * run.tile_steps / share.run(run.tiles));
+      float* to = inner + ((size_t)part * p.n_tokens + tile.first) * RP + row * 4;
 #pragma unroll
-      for (int c = 0; c < kStep; c += 16) {
+      for (int c = 0; c < RP; c += 16) {
         float v[16];
-        from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + c);
+        from_tensor_memory(v, tmem + ((warp - 4) * 32 << 16) + (n & 1) * RP + c);
         loads_done();
+        if (row < tile.count) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t piece = at + (c / 8 + h) * (kBigTile * 16) + row * 16;
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece) : "memory");
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float2 b = Half<E>::widen(w[j]);
-            w[j] = Half<E>::narrow(fmaf(v[8 * h + 2 * j], back, b.x), fmaf(v[8 * h + 2 * j + 1], back, b.y));
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(piece), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(to + (size_t)(c + i) * tile.count) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
       before_sync();
       __syncwarp();
-      if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const uint32_t c = (lane >> 3) + 4 * h;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(at + c * (kBigTile * 16) + (quarter * 32 + 8 * j + (lane & 7)) * 16)
-                       : "memory");
-          if (to[j] && column + c * 8 < p.out_dim) *reinterpret_cast<uint4*>(to[j] + column + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) barrier_arrive(shared_address(&drained[s]));
+      if (lane == 0) barrier_arrive(shared_address(&taken[n & 1]));
     }
   } else if (lane == 0) {
-    bool ok = barrier_wait(shared_address(&terms), 0);
-    for (uint32_t i = 0; ok && i < steps; i++) {
-      const uint32_t s = i % kStages, at = ring + s * S::kStageBytes + kRowsBytes;
-      ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) &&
-           (i < 2 || barrier_wait(shared_address(&taken[i & 1]), (i / 2 - 1) & 1));
-      if (!ok) break;
-      after_sync();
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
+      if (n >= 2 && !barrier_wait(shared_address(&taken[n & 1]), (n / 2 - 1) & 1)) break;
+      bool add = false;
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        const uint32_t s = i % kStages, at = ring + s * S::kDownStage;
+        if (!(ok = barrier_wait(shared_address(&full[s]), i / kStages & 1))) break;
+        order_for_tensor_cores();
+        after_sync();
 #pragma unroll
-      for (int t = 0; t < 2; t++)
-#pragma unroll
-        for (int k = 0; k < RP / 16; k++)
-          multiply(tmem + (i & 1) * kStep, operand(term + t * S::kTermBytes + k * 2 * kBigTile * 16, kBigTile * 16),
-                   operand(at + k * 2 * kStep * 16, kStep * 16), instruction<E>(kStep), t > 0 || k > 0);
-      arrive_behind_products(shared_address(&product[i & 1]));
+        for (int q = 0; q < kStep / 16; q++) {
+          multiply(tmem + (n & 1) * RP, operand(at + q * 32), operand(at + kRowsBytes + q * 32), instruction<E>(RP), add);
+          add = true;
+        }
+        arrive_behind_products(shared_address(&empty[s]));
+      }
+      if (ok) arrive_behind_products(shared_address(&ready[n & 1]));
     }
   }
   before_sync();
   __syncthreads();
   after_sync();
   if (warp == 8) free_tensor_memory<kColumns>(tmem);
+}
+
+template <typename E, int RP>
+__global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
+    adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, BigShare down_share, BigShare share) {
+  using S = BigShape<RP>;
+  constexpr int kStages = S::kUpStages, kColumns = 2 * kStep;
+  extern __shared__ unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kStages], drained[kStages], product[2], taken[2], terms, tops;
+  __shared__ uint32_t tmem_slot;
+  __shared__ float top_of[2][kBigTile];
+  __shared__ Tile tiles[kMostTiles];
+  // the launch ahead (the first product) started behind everything that wrote base, up and the plan
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Run run = find_run<kUpThreads>(p, share, p.out != p.base, tiles);
+  if (run.count == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      barrier_init(shared_address(&full[i]), kProducers);
+      barrier_init(shared_address(&drained[i]), 8);
+    }
+    for (int i = 0; i < 2; i++) {
+      barrier_init(shared_address(&product[i]), 1);
+      barrier_init(shared_address(&taken[i]), 8);
+    }
+    barrier_init(shared_address(&terms), 256);
+    barrier_init(shared_address(&tops), 256);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) tensor_memory<kColumns>(&tmem_slot);
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = tmem_slot, ring = aligned_shared(smem), term = ring + kStages * S::kUpStage;
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+
+  if (warp < 4) {
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
+      const Tile tile = tiles[n];
+      if (tile.group == p.n_groups) break;  // these come last
+      RowCopies base;
+      base.set(p.base, p.base_stride, p, tile);
+      const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        const uint32_t s = i % kStages;
+        if (i >= kStages && !(ok = barrier_wait(shared_address(&drained[s]), (i / kStages - 1) & 1))) break;
+        const uint32_t to = ring + s * S::kUpStage, column = k * kStep;
+        base.issue(to, column, p.out_dim);
+        copy_matrix<kStep, RP / 8>(to + kRowsBytes, up, p.rank, column, p.out_dim, 0, p.rank);
+        arrive_behind_copies(shared_address(&full[s]));
+      }
+    }
+    copies_done();
+  } else if (warp < 12) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const uint32_t out_piece = half * 4 + (lane & 3), out_row = quarter * 32 + (lane >> 2 & 1) * 4 + (lane >> 3);
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
+      const Tile tile = tiles[n];
+      if (tile.group == p.n_groups) {  // no adapter
+        const uint16_t* base = static_cast<const uint16_t*>(p.base);
+        const uint32_t begin = run.from(n) * kStep, end = min(p.out_dim, run.to(n) * kStep);
+        for (uint32_t m = warp - 4; m < tile.count; m += 8) {
+          const int t = token_at(p, tile, m);
+          if (t < 0) continue;
+          for (uint32_t c = begin + lane * 8; c < end; c += 256)
+            *reinterpret_cast<uint4*>(out + (long long)t * p.out_stride + c) =
+                *reinterpret_cast<const uint4*>(base + (long long)t * p.base_stride + c);
+        }
+        continue;
+      }
+      float back;
+      {  // half of the token's rank products a thread: added up, scaled so that the token's largest is in [1, 2), in two terms
+        constexpr int R = RP / 2;
+        const float scale = p.scale ? p.scale[tile.group] : 1.f;
+        const uint32_t per = down_share.run(run.tiles);
+        const unsigned long long at = (unsigned long long)(run.first + n) * down_share.tile_steps;
+        const uint32_t parts = (uint32_t)((at + down_share.tile_steps - 1) / per - at / per) + 1;
+        const float* from = inner + (size_t)tile.first * RP + (size_t)half * R * tile.count + min(row, tile.count - 1) * 4;
+        float u[R], top = 0.f;
+#pragma unroll
+        for (int c = 0; c < R; c++) u[c] = 0.f;
+        for (uint32_t m = 0; m < parts; m++, from += (size_t)p.n_tokens * RP) {
+#pragma unroll
+          for (int c = 0; c < R; c += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + (size_t)c * tile.count));
+            u[c] += v.x, u[c + 1] += v.y, u[c + 2] += v.z, u[c + 3] += v.w;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < R; c++) {
+          u[c] *= scale;
+          top = fmaxf(top, fabsf(u[c]));
+        }
+        top_of[half][row] = top;
+        barrier_arrive(shared_address(&tops));
+        if (!(ok = barrier_wait(shared_address(&tops), n & 1))) break;
+        const float s = unit_scale(fmaxf(top, top_of[half ^ 1][row]));
+        back = 1.f / s;
+#pragma unroll
+        for (int c = 0; c < R; c += 8) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float a = u[c + 2 * j] * s, b = u[c + 2 * j + 1] * s;
+            hi[j] = Half<E>::narrow(a, b);
+            const float2 h = Half<E>::widen(hi[j]);
+            lo[j] = Half<E>::narrow(isinf(h.x) ? 0.f : a - h.x, isinf(h.y) ? 0.f : b - h.y);
+          }
+          const uint32_t q = (half * R + c) / 8, q2 = q + RP / 8;  // the second terms follow the first
+          const uint32_t to = term + q / 8 * (kBigTile * 128) + piece_at(row, q % 8);
+          const uint32_t to2 = term + q2 / 8 * (kBigTile * 128) + piece_at(row, q2 % 8);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to2), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+        }
+      }
+      order_for_tensor_cores();
+      barrier_arrive(shared_address(&terms));
+      uint16_t* to[4];  // on the way out the thread has one piece of four rows
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int t = token_at(p, tile, out_row + 8 * j);
+        to[j] = t < 0 ? nullptr : out + (long long)t * p.out_stride + out_piece * 8;
+      }
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        const uint32_t s = i % kStages, at = ring + s * S::kUpStage, column = k * kStep;
+        ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) && barrier_wait(shared_address(&product[i & 1]), i / 2 & 1);
+        if (!ok) break;
+        after_sync();
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          float v[16];
+          from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + half * 32 + c * 8);
+          uint32_t w[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[h][0]), "=r"(w[h][1]), "=r"(w[h][2]), "=r"(w[h][3])
+                         : "r"(at + piece_at(row, half * 4 + c + h))
+                         : "memory");
+          loads_done();
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float2 b = Half<E>::widen(w[h][j]);
+              w[h][j] = Half<E>::narrow(fmaf(v[8 * h + 2 * j], back, b.x), fmaf(v[8 * h + 2 * j + 1], back, b.y));
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + piece_at(row, half * 4 + c + h)), "r"(w[h][0]),
+                         "r"(w[h][1]), "r"(w[h][2]), "r"(w[h][3])
+                         : "memory");
+          }
+        }
+        before_sync();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(at + piece_at(out_row + 8 * j, out_piece))
+                       : "memory");
+          if (to[j] && column + out_piece * 8 < p.out_dim) *reinterpret_cast<uint4*>(to[j] + column) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_address(&drained[s]));
+      }
+    }
+  } else if (lane == 0) {
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
+      if (tiles[n].group == p.n_groups) break;
+      if (!(ok = barrier_wait(shared_address(&terms), n & 1))) break;
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        const uint32_t s = i % kStages, at = ring + s * S::kUpStage + kRowsBytes;
+        ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) &&
+             (i < 2 || barrier_wait(shared_address(&taken[i & 1]), (i / 2 - 1) & 1));
+        if (!ok) break;
+        order_for_tensor_cores();
+        after_sync();
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < RP / 16; r++) {
+            const int q = t * (RP / 16) + r;  // sixteen ranks of a term
+            multiply(tmem + (i & 1) * kStep, operand(term + q / 4 * (kBigTile * 128) + q % 4 * 32),
+                     operand(at + r / 4 * (kStep * 128) + r % 4 * 32), instruction<E>(kStep), q > 0);
+          }
+        arrive_behind_products(shared_address(&product[i & 1]));
+      }
+    }
+  }
+  before_sync();
+  __syncthreads();
+  after_sync();
+  if (warp == 12) free_tensor_memory<kColumns>(tmem);
 }
 
 template <typename E, int RP>
@@ -761,17 +868,23 @@ cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t str
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// How a batch of prompts is split: CTAs a tile of the first and of the second product.
+// Runs of both products.  At most: every group may end in a tile of its own.
 struct BigSplit {
-  uint32_t tiles, splits, slices;
+  BigShare down, up;
+  uint32_t parts;  // partial sums a tile has, at most
 };
 BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t dim, uint32_t out_dim) {
-  constexpr uint32_t kSlots = 2 * 148;
+  constexpr uint32_t kSlots = 2 * 148, kMostParts = 8, kLeastUp = 4;
+  const uint32_t most_tiles = n_tokens / kBigTile + std::min(n_groups + 1, n_tokens), tiles = (n_tokens + kBigTile - 1) / kBigTile;
+  const uint32_t grid = std::max(kSlots, (most_tiles + kMostTiles - 4) / (kMostTiles - 3));
+  auto over = [](unsigned long long a, unsigned long long b) { return (uint32_t)((a + b - 1) / b); };
   BigSplit b;
-  b.tiles = n_tokens / kBigTile + std::min(n_groups + 1, n_tokens);  // at most: every group may end in a tile of its own
-  const uint32_t k = (dim + kStep - 1) / kStep, n = (out_dim + kStep - 1) / kStep;
-  b.splits = std::min({(kSlots + b.tiles - 1) / b.tiles, k, 8u});
-  b.slices = std::min((2 * kSlots + b.tiles - 1) / b.tiles, n);
+  b.down.tile_steps = over(dim, kStep);
+  b.up.tile_steps = over(out_dim, kStep);
+  b.down.grid = b.up.grid = grid;
+  b.down.least = std::max(over((unsigned long long)tiles * b.down.tile_steps, grid), over(b.down.tile_steps, kMostParts - 1));
+  b.up.least = std::min(kLeastUp, b.up.tile_steps);
+  b.parts = over(b.down.tile_steps, b.down.least) + 1;
   return b;
 }
 int padded_rank(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
@@ -794,22 +907,22 @@ cudaError_t big_launch(const AdapterParams& p, float* inner, cudaStream_t stream
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(b.tiles * b.splits);
+  cfg.gridDim = dim3(b.down.grid);
   cfg.blockDim = dim3(kDownThreads);
   cfg.dynamicSmemBytes = S::kDownShared;
-  e = cudaLaunchKernelEx(&cfg, down, p, inner, b.splits);
+  e = cudaLaunchKernelEx(&cfg, down, p, inner, b.down);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(b.tiles * b.slices);
+  cfg.gridDim = dim3(b.up.grid);
   cfg.blockDim = dim3(kUpThreads);
   cfg.dynamicSmemBytes = S::kUpShared;
-  return cudaLaunchKernelEx(&cfg, up, p, static_cast<const float*>(inner), b.splits, b.slices);
+  return cudaLaunchKernelEx(&cfg, up, p, static_cast<const float*>(inner), b.down, b.up);
 }
 
 }  // namespace
 
 size_t adapter_scratch_bytes(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t dim, uint32_t out_dim) {
   if (!big_batch(n_tokens, n_groups)) return 0;
-  return (size_t)big_split(n_tokens, n_groups, dim, out_dim).splits * n_tokens * padded_rank(rank) * sizeof(float);
+  return (size_t)big_split(n_tokens, n_groups, dim, out_dim).parts * n_tokens * padded_rank(rank) * sizeof(float);
 }
 
 cudaError_t adapter_stalled(uint32_t* count) { return cudaMemcpyFromSymbol(count, g_stalled, sizeof(*count)); }
