@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p) {
 // the unit takes, split every line over eight and cost 2.5 times the time.)
 
 constexpr int kBigTile = 128;
-constexpr int kStep = 64;                                   // columns a step
+constexpr int kStep = 128;                                  // columns a step
+constexpr int kBlock64 = kBigTile * 128;                    // 64 columns of a tile's rows
 constexpr int kRowsBytes = kBigTile * kStep * 2;            // x or base of a step
 constexpr int kProducers = 128;
 constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, multiply
@@ -428,10 +429,15 @@ struct RowCopies {
   }
   static __device__ __forceinline__ uint32_t place(int i) { return 4 * ((threadIdx.x >> 5) + 4 * i) + (threadIdx.x >> 3 & 3); }
   __device__ __forceinline__ void issue(uint32_t to, uint32_t column, uint32_t end) const {
-    const bool live = column + (threadIdx.x & 7) * 8 < end;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (row[i]) copy16(to + piece_at(place(i), threadIdx.x & 7), live ? row[i] + column : row[i], live);
+    for (int i = 0; i < 8; i++) {
+      if (!row[i]) continue;
+#pragma unroll
+      for (int b = 0; b < kStep / 64; b++) {
+        const bool live = column + b * 64 + (threadIdx.x & 7) * 8 < end;
+        copy16(to + b * kBlock64 + piece_at(place(i), threadIdx.x & 7), live ? row[i] + column + b * 64 : row[i], live);
+      }
+    }
   }
 };
 
@@ -451,12 +457,12 @@ __device__ __forceinline__ void copy_matrix(uint32_t to, const uint16_t* from, s
 
 template <int RP>
 struct BigShape {
-  static constexpr int kDownStage = kRowsBytes + RP * 128;                      // x, down
+  static constexpr int kDownStage = kRowsBytes + RP * kStep * 2;                // x, down
   static constexpr int kUpStage = kRowsBytes + (RP + 63) / 64 * kStep * 128;    // base, up
   static constexpr int kTermBytes = (2 * RP + 63) / 64 * kBigTile * 128;        // the rank products: first terms, then second
-  // two CTAs an SM up to rank 64; one above
-  static constexpr int kDownStages = 4;
-  static constexpr int kUpStages = RP <= 64 ? 3 : 4;
+  // one CTA an SM, as many stages as fit
+  static constexpr int kDownStages = RP <= 32 ? 5 : RP <= 64 ? 4 : 3;
+  static constexpr int kUpStages = RP <= 64 ? 4 : 2;
   static constexpr int kDownShared = kDownStages * kDownStage + 1024;
   static constexpr int kUpShared = kUpStages * kUpStage + kTermBytes + 1024;
 };
@@ -542,7 +548,7 @@ __device__ Run find_run(const AdapterParams& p, const BigShare& share, bool bare
 // inner[part] = x rows of the tile times a run of columns of `down`; a tile's RP products a token lie as
 // [RP / 4][tokens][4], so that one token a thread writes and reads whole lines.
 template <typename E, int RP>
-__global__ void __launch_bounds__(kDownThreads, RP <= 64 ? 2 : 1) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, BigShare share) {
+__global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, BigShare share) {
   using S = BigShape<RP>;
   constexpr int kStages = S::kDownStages, kColumns = 2 * RP;
   extern __shared__ unsigned char smem[];
@@ -584,7 +590,7 @@ __global__ void __launch_bounds__(kDownThreads, RP <= 64 ? 2 : 1) adapter_down_k
         if (i >= kStages && !(ok = barrier_wait(shared_address(&empty[s]), (i / kStages - 1) & 1))) break;
         const uint32_t to = ring + s * S::kDownStage, column = k * kStep;
         x.issue(to, column, p.dim);
-        copy_matrix<RP, 8>(to + kRowsBytes, down, p.dim, 0, p.rank, column, p.dim);
+        copy_matrix<RP, kStep / 8>(to + kRowsBytes, down, p.dim, 0, p.rank, column, p.dim);
         arrive_behind_copies(shared_address(&full[s]));
       }
     }
@@ -625,7 +631,8 @@ __global__ void __launch_bounds__(kDownThreads, RP <= 64 ? 2 : 1) adapter_down_k
         after_sync();
 #pragma unroll
         for (int q = 0; q < kStep / 16; q++) {
-          multiply(tmem + (n & 1) * RP, operand(at + q * 32), operand(at + kRowsBytes + q * 32), instruction<E>(RP), add);
+          multiply(tmem + (n & 1) * RP, operand(at + q / 4 * kBlock64 + q % 4 * 32),
+                   operand(at + kRowsBytes + q / 4 * (RP * 128) + q % 4 * 32), instruction<E>(RP), add);
           add = true;
         }
         arrive_behind_products(shared_address(&empty[s]));
@@ -640,7 +647,7 @@ __global__ void __launch_bounds__(kDownThreads, RP <= 64 ? 2 : 1) adapter_down_k
 }
 
 template <typename E, int RP>
-__global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kUpThreads, 1)
     adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, BigShare down_share, BigShare share) {
   using S = BigShape<RP>;
   constexpr int kStages = S::kUpStages, kColumns = 2 * kStep;
@@ -698,7 +705,8 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
   } else if (warp < 12) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-    const uint32_t out_piece = half * 4 + (lane & 3), out_row = quarter * 32 + (lane >> 2 & 1) * 4 + (lane >> 3);
+    static_assert(kStep == 128, "a half of the step's columns is one block of 64");
+    const uint32_t block = half * kBlock64, out_piece = lane & 7, out_row = quarter * 32 + (lane >> 3);
     uint32_t i = 0;
     bool ok = true;
     for (uint32_t n = 0; ok && n < run.count; n++) {
@@ -754,19 +762,19 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
             lo[j] = Half<E>::narrow(isinf(h.x) ? 0.f : a - h.x, isinf(h.y) ? 0.f : b - h.y);
           }
           const uint32_t q = (half * R + c) / 8, q2 = q + RP / 8;  // the second terms follow the first
-          const uint32_t to = term + q / 8 * (kBigTile * 128) + piece_at(row, q % 8);
-          const uint32_t to2 = term + q2 / 8 * (kBigTile * 128) + piece_at(row, q2 % 8);
+          const uint32_t to = term + q / 8 * kBlock64 + piece_at(row, q % 8);
+          const uint32_t to2 = term + q2 / 8 * kBlock64 + piece_at(row, q2 % 8);
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to2), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
         }
       }
       order_for_tensor_cores();
       barrier_arrive(shared_address(&terms));
-      uint16_t* to[4];  // on the way out the thread has one piece of four rows
+      uint16_t* to[8];  // on the way out the thread has one piece of eight rows
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int t = token_at(p, tile, out_row + 8 * j);
-        to[j] = t < 0 ? nullptr : out + (long long)t * p.out_stride + out_piece * 8;
+      for (int j = 0; j < 8; j++) {
+        const int t = token_at(p, tile, out_row + 4 * j);
+        to[j] = t < 0 ? nullptr : out + (long long)t * p.out_stride + half * 64 + out_piece * 8;
       }
       for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
         const uint32_t s = i % kStages, at = ring + s * S::kUpStage, column = k * kStep;
@@ -774,15 +782,15 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
         if (!ok) break;
         after_sync();
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
+        for (int c = 0; c < 8; c += 2) {
           float v[16];
-          from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + half * 32 + c * 8);
+          from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + half * 64 + c * 8);
           uint32_t w[2][4];
 #pragma unroll
           for (int h = 0; h < 2; h++)
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                          : "=r"(w[h][0]), "=r"(w[h][1]), "=r"(w[h][2]), "=r"(w[h][3])
-                         : "r"(at + piece_at(row, half * 4 + c + h))
+                         : "r"(at + block + piece_at(row, c + h))
                          : "memory");
           loads_done();
 #pragma unroll
@@ -792,7 +800,7 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
               const float2 b = Half<E>::widen(w[h][j]);
               w[h][j] = Half<E>::narrow(fmaf(v[8 * h + 2 * j], back, b.x), fmaf(v[8 * h + 2 * j + 1], back, b.y));
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + piece_at(row, half * 4 + c + h)), "r"(w[h][0]),
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + block + piece_at(row, c + h)), "r"(w[h][0]),
                          "r"(w[h][1]), "r"(w[h][2]), "r"(w[h][3])
                          : "memory");
           }
@@ -801,13 +809,13 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
         __syncwarp();
         if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
           uint32_t w[4];
           asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(at + piece_at(out_row + 8 * j, out_piece))
+                       : "r"(at + block + piece_at(out_row + 4 * j, out_piece))
                        : "memory");
-          if (to[j] && column + out_piece * 8 < p.out_dim) *reinterpret_cast<uint4*>(to[j] + column) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (to[j] && column + half * 64 + out_piece * 8 < p.out_dim) *reinterpret_cast<uint4*>(to[j] + column) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncwarp();
         if (lane == 0) barrier_arrive(shared_address(&drained[s]));
@@ -831,7 +839,7 @@ __global__ void __launch_bounds__(kUpThreads, RP <= 64 ? 2 : 1)
 #pragma unroll
           for (int r = 0; r < RP / 16; r++) {
             const int q = t * (RP / 16) + r;  // sixteen ranks of a term
-            multiply(tmem + (i & 1) * kStep, operand(term + q / 4 * (kBigTile * 128) + q % 4 * 32),
+            multiply(tmem + (i & 1) * kStep, operand(term + q / 4 * kBlock64 + q % 4 * 32),
                      operand(at + r / 4 * (kStep * 128) + r % 4 * 32), instruction<E>(kStep), q > 0);
           }
         arrive_behind_products(shared_address(&product[i & 1]));
@@ -874,7 +882,7 @@ struct BigSplit {
   uint32_t parts;  // partial sums a tile has, at most
 };
 BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t dim, uint32_t out_dim) {
-  constexpr uint32_t kSlots = 2 * 148, kMostParts = 8, kLeastUp = 4;
+  constexpr uint32_t kSlots = 148, kMostParts = 8, kLeastUp = 2;
   const uint32_t most_tiles = n_tokens / kBigTile + std::min(n_groups + 1, n_tokens), tiles = (n_tokens + kBigTile - 1) / kBigTile;
   const uint32_t grid = std::max(kSlots, (most_tiles + kMostTiles - 4) / (kMostTiles - 3));
   auto over = [](unsigned long long a, unsigned long long b) { return (uint32_t)((a + b - 1) / b); };
