@@ -17,7 +17,6 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kBlock = kWarps * 32;
-constexpr int kCluster = 8;   // CTAs that share a tile of tokens
 constexpr int kTile = 16;     // tokens of a tile: the rows of one matrix instruction
 
 template <typename E>
@@ -122,206 +121,6 @@ __device__ Tile find_tile(const int32_t* offsets, uint32_t n_groups, uint32_t n_
   return found;
 }
 
-// RP: rank rounded up to 8, 16, 32, 64 or 128.
-template <typename E, int RP, bool VECTOR>
-__global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  constexpr int RT = RP / 8;                 // tiles of 8 ranks
-  constexpr int KR = RP < 16 ? 16 : RP;      // ranks as the second product's depth
-  extern __shared__ __align__(16) unsigned char smem[];
-  using Part = float[kTile][RP];
-  using Inner = uint16_t[kTile][KR + 8];
-  Part* part = reinterpret_cast<Part*>(smem);                            // [kWarps] of each warp, then [0]: of the CTA
-  Inner* inner = reinterpret_cast<Inner*>(smem + kWarps * sizeof(Part)); // [2] the two terms
-  __shared__ float back[kTile];
-  __shared__ int32_t token[kTile];
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t member = cluster.block_rank();
-  const Tile tile = find_tile<kTile, kBlock>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / kCluster);
-  if (tile.count == 0) return;  // of the whole cluster
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  if (threadIdx.x < kTile) {
-    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
-    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
-  }
-  __syncthreads();
-  const uint16_t* base = static_cast<const uint16_t*>(p.base);
-  uint16_t* out = static_cast<uint16_t*>(p.out);
-  const uint32_t n_slice = (p.out_dim + kCluster * 32 - 1) / (kCluster * 32) * 32;
-  const uint32_t n_begin = member * n_slice, n_end = min(p.out_dim, n_begin + n_slice);
-
-  if (tile.group == p.n_groups) {  // no adapter
-    if (out == base) return;
-    for (uint32_t m = warp; m < tile.count; m += kWarps) {
-      if (token[m] < 0) continue;
-      const uint16_t* from = base + (long long)token[m] * p.base_stride;
-      uint16_t* to = out + (long long)token[m] * p.out_stride;
-      for (uint32_t n = n_begin + lane * 8; n < n_end; n += 256) {
-        if (VECTOR && n + 8 <= n_end) {
-          *reinterpret_cast<uint4*>(to + n) = *reinterpret_cast<const uint4*>(from + n);
-        } else {
-          for (uint32_t i = n; i < min(n + 8, n_end); i++) to[i] = from[i];
-        }
-      }
-    }
-    return;
-  }
-
-  // first product: every CTA a slice of dim, its warps 32 of it at a time
-  {
-    const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
-    const uint16_t* x = static_cast<const uint16_t*>(p.x);
-    const uint32_t k_slice = (p.dim + kCluster * 32 - 1) / (kCluster * 32) * 32;
-    const uint32_t k_end = min(p.dim, (member + 1) * k_slice);
-    const int t0 = token[g], t1 = token[g + 8];
-    float acc[RT][4] = {};
-    for (uint32_t k = member * k_slice + warp * 32; k < k_end; k += kWarps * 32) {
-      const int at = (int)k + (int)c * 8, valid = (int)p.dim - at;
-      uint32_t r0[4] = {}, r1[4] = {};
-      if (t0 >= 0 && valid > 0) load_words<4, VECTOR>(r0, x + (long long)t0 * p.x_stride + at, valid);
-      if (t1 >= 0 && valid > 0) load_words<4, VECTOR>(r1, x + (long long)t1 * p.x_stride + at, valid);
-      const uint32_t a0[4] = {r0[0], r1[0], r0[1], r1[1]}, a1[4] = {r0[2], r1[2], r0[3], r1[3]};
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-        uint32_t b[4] = {};
-        const uint32_t rank = r * 8 + g;
-        if (rank < p.rank && valid > 0) load_words<4, VECTOR>(b, down + (size_t)rank * p.dim + at, valid);
-        Half<E>::mma(acc[r], a0, b[0], b[1]);
-        Half<E>::mma(acc[r], a1, b[2], b[3]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < RT; r++) {
-      *reinterpret_cast<float2*>(&part[warp][g][r * 8 + c * 2]) = make_float2(acc[r][0], acc[r][1]);
-      *reinterpret_cast<float2*>(&part[warp][g + 8][r * 8 + c * 2]) = make_float2(acc[r][2], acc[r][3]);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * RP; i += kBlock) {
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) sum += (&part[w][0][0])[i];
-      (&part[0][0][0])[i] = sum;
-    }
-  }
-  cluster.sync();
-  // the CTAs' sums, in their order; scaled to the row's largest so that both 16-bit terms keep their bits
-  {
-    const float scale = p.scale ? p.scale[tile.group] : 1.f;
-    for (int i = threadIdx.x; i < kTile * RP; i += kBlock) {
-      float sum = 0.f;
-#pragma unroll
-      for (int m = 0; m < kCluster; m++) sum += cluster.map_shared_rank(&part[0][0][0], m)[i];
-      (&part[1][0][0])[i] = sum * scale;
-    }
-    __syncthreads();
-    for (int m = warp; m < kTile; m += kWarps) {
-      float top = 0.f;
-      for (int r = lane; r < RP; r += 32) top = fmaxf(top, fabsf(part[1][m][r]));
-#pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-      const float s = unit_scale(top);
-      if (lane == 0) back[m] = 1.f / s;
-      for (int r = lane * 2; r < KR; r += 64) {
-        const float u0 = r < RP ? part[1][m][r] * s : 0.f, u1 = r < RP ? part[1][m][r + 1] * s : 0.f;
-        const uint32_t hi = Half<E>::narrow(u0, u1);
-        const float2 h = Half<E>::widen(hi);
-        // what the first term leaves; nothing where the first is infinite
-        const uint32_t lo = Half<E>::narrow(isinf(h.x) ? 0.f : u0 - h.x, isinf(h.y) ? 0.f : u1 - h.y);
-        *reinterpret_cast<uint32_t*>(&inner[0][m][r]) = hi;
-        *reinterpret_cast<uint32_t*>(&inner[1][m][r]) = lo;
-      }
-    }
-  }
-  cluster.sync();  // also: nobody leaves while its sums are being read
-
-  // second product: every CTA a slice of out_dim, its warps 32 of it at a time.  Column 2c + b of the
-  // q-th of four matrix tiles is output 8c + 2q + b, so that a lane ends with 8 consecutive outputs.
-  {
-    const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
-    constexpr int KS = KR >= 32 ? KR / 32 : 1;   // steps of 32 (16) ranks
-    constexpr int W = KR >= 32 ? 4 : 2;          // words a lane has of one
-    uint32_t u[2][2][KS][W];                     // term, half of the tile
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int o = 0; o < 2; o++)
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-          load_words<W, true>(u[h][o][s], &inner[h][g + 8 * o][(s * 4 + c) * 2 * W], 2 * W);
-    for (uint32_t n0 = n_begin + warp * 32; n0 < n_end; n0 += kWarps * 32) {
-      float acc[4][4] = {};
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const uint32_t n = n0 + (g >> 1) * 8 + q * 2 + (g & 1);
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-          uint32_t b[W] = {};
-          const int at = (s * 4 + (int)c) * 2 * W, valid = (int)p.rank - at;
-          if (n < n_end && valid > 0) load_words<W, VECTOR>(b, up + (size_t)n * p.rank + at, valid);
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int w = 0; w < W; w += 2) {
-              const uint32_t a[4] = {u[h][0][s][w], u[h][1][s][w], u[h][0][s][w + 1], u[h][1][s][w + 1]};
-              Half<E>::mma(acc[q], a, b[w], b[w + 1]);
-            }
-        }
-      }
-      const int at = (int)(n0 + c * 8), valid = (int)n_end - at;
-#pragma unroll
-      for (int o = 0; o < 2; o++) {
-        const int t = token[g + 8 * o];
-        if (t < 0 || valid <= 0) continue;
-        uint32_t in[4];
-        load_words<4, VECTOR>(in, base + (long long)t * p.base_stride + at, valid);
-        const float s = back[g + 8 * o];
-        uint32_t y[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const float2 v = Half<E>::widen(in[q]);
-          y[q] = Half<E>::narrow(fmaf(acc[q][2 * o], s, v.x), fmaf(acc[q][2 * o + 1], s, v.y));
-        }
-        uint16_t* to = out + (long long)t * p.out_stride + at;
-        if (VECTOR && valid >= 8) {
-          *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++)
-            if (i < valid) to[i] = (uint16_t)(y[i / 2] >> (i & 1 ? 16 : 0));
-        }
-      }
-    }
-  }
-}
-
-// ------------------------------------------------------------------------------------
-// prompts: tiles of 128 tokens on the 5th-generation tensor cores
-// ------------------------------------------------------------------------------------
-// Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
-// partial sums in the workspace; the second adds those up, splits them into two 16-bit terms and multiplies
-// them with `up`, adding `base` on the way out.  In both a tile is so many steps of 64 columns, the tiles of the
-// batch stand one behind the other, and every CTA of a full GPU takes the same number of consecutive
-// steps, so that no number of tiles leaves part of the GPU idle; where a CTA's run starts or ends inside a tile
-// of the first product, the tile has one more partial sum.
-// Steps go through a ring of stages in shared memory: four warps copy (token rows lie anywhere, so 16
-// bytes a thread), one thread issues the matrix instructions, the other warps take the products out of
-// tensor memory.
-//
-// Operands lie in shared memory in rows of 128 bytes whose 16-byte pieces are exchanged by row (piece c
-// of row r at c ^ (r % 8)), as the matrix unit reads them: a line of global memory is a line there, and
-// one token a thread reads `base` without bank conflicts.  (Blocks of 8 rows x 16 bytes, the other layout
-// the unit takes, split every line over eight and cost 2.5 times the time.)
-
-constexpr int kBigTile = 128;
-constexpr int kStep = 128;                                  // columns a step
-constexpr int kBlock64 = kBigTile * 128;                    // 64 columns of a tile's rows
-constexpr int kRowsBytes = kBigTile * kStep * 2;            // x or base of a step
-constexpr int kProducers = 128;
-constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, multiply
-constexpr int kUpThreads = kProducers + 256 + 32;
-constexpr int kMostTiles = 36;                              // a CTA's run touches
-
 __device__ unsigned int g_stalled;  // waits that ran out
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -352,6 +151,300 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     }
   }
 }
+
+// ------------------------------------------------------------------------------------
+// single tokens: a cluster of CTAs has a tile of 16 tokens
+// ------------------------------------------------------------------------------------
+// Bound by the adapters' matrices and, with few tokens, by the chain plan - tile - x, down - up.  Every CTA of
+// the cluster has a slice of dim and, later, of out_dim; the CTAs hand one another their partial rank products
+// through distributed shared memory.  `up` does not wait for those: a bulk copy brings the slice
+// (what fits) into shared memory meanwhile.  The matrix instructions take the columns of a product in any
+// order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.
+
+constexpr int kMostCluster = 8;
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// RP: rank rounded up to 8, 16, 32, 64 or 128.
+template <int RP>
+struct SmallShape {
+  static constexpr int kWarpRanks = RP < 32 ? RP : 32;          // ranks a warp has in the first product
+  static constexpr int kRankGroups = RP / kWarpRanks;
+  static constexpr int kDepthGroups = kWarps / kRankGroups;     // warps that share a slice of dim
+  static constexpr int kDepth = RP < 16 ? 16 : RP;              // ranks as the second product's depth
+  static constexpr int kPart = kDepthGroups * kTile * RP * 4;
+  static constexpr int kInner = 2 * kTile * (kDepth + 8) * 2;
+  static constexpr int kShared = kPart + kInner;                // and what is held of `up`
+};
+
+template <typename E, int RP, bool VECTOR>
+__global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32_t up_room) {
+  using S = SmallShape<RP>;
+  constexpr int KR = S::kDepth;
+  extern __shared__ __align__(128) unsigned char smem[];
+  using Inner = uint16_t[kTile][KR + 8];
+  float* part = reinterpret_cast<float*>(smem);                              // [depth group][token][rank]
+  Inner* inner = reinterpret_cast<Inner*>(smem + S::kPart);                  // [term]
+  uint16_t* up_here = reinterpret_cast<uint16_t*>(smem + S::kPart + S::kInner);
+  __shared__ float back[kTile];
+  __shared__ int32_t token[kTile];
+  __shared__ __align__(8) uint64_t up_landed;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t member = cluster.block_rank(), members = cluster.num_blocks();
+  if (threadIdx.x == 0) {
+    barrier_init(shared_address(&up_landed), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const Tile tile = find_tile<kTile, kBlock>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / members);
+  if (tile.count == 0) return;  // of the whole cluster
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const uint32_t n_slice = (p.out_dim + members * 32 - 1) / (members * 32) * 32;
+  const uint32_t n_begin = min(p.out_dim, member * n_slice), n_end = min(p.out_dim, n_begin + n_slice);
+  const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
+  const bool bare = tile.group == p.n_groups;
+  const uint32_t held = VECTOR && !bare ? min(n_end - n_begin, up_room / 2 / p.rank) : 0;  // rows of `up` to bring here
+  if (threadIdx.x == 0 && held) {
+    const uint32_t bytes = held * p.rank * 2;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&up_landed)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(up_here)),
+                 "l"(up + (size_t)n_begin * p.rank), "r"(bytes), "r"(shared_address(&up_landed))
+                 : "memory");
+    if (held < n_end - n_begin)  // the rest on its way from HBM
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(up + (size_t)(n_begin + held) * p.rank),
+                   "r"((n_end - n_begin - held) * p.rank * 2)
+                   : "memory");
+  }
+  if (threadIdx.x < kTile) {
+    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
+    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
+  }
+  __syncthreads();
+  const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+
+  if (bare) {  // no adapter
+    if (out == base) return;
+    for (uint32_t m = warp; m < tile.count; m += kWarps) {
+      if (token[m] < 0) continue;
+      const uint16_t* from = base + (long long)token[m] * p.base_stride;
+      uint16_t* to = out + (long long)token[m] * p.out_stride;
+      for (uint32_t n = n_begin + lane * 8; n < n_end; n += 256) {
+        if (VECTOR && n + 8 <= n_end) {
+          *reinterpret_cast<uint4*>(to + n) = *reinterpret_cast<const uint4*>(from + n);
+        } else {
+          for (uint32_t i = n; i < min(n + 8, n_end); i++) to[i] = from[i];
+        }
+      }
+    }
+    return;
+  }
+
+  // first product: every CTA a slice of dim, 32 of it a warp at a time, several such loads in flight
+  {
+    const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
+    const uint16_t* x = static_cast<const uint16_t*>(p.x);
+    const uint32_t k_slice = (p.dim + members * 32 - 1) / (members * 32) * 32;
+    const uint32_t k_end = min(p.dim, (member + 1) * k_slice);
+    const uint32_t depth_group = warp % S::kDepthGroups, rank0 = warp / S::kDepthGroups * S::kWarpRanks;
+    const int t0 = token[g], t1 = token[g + 8];
+    constexpr int RT = S::kWarpRanks / 8, kFlight = 2;
+    constexpr uint32_t kPace = S::kDepthGroups * 32;
+    float acc[RT][4] = {};
+    for (uint32_t k0 = member * k_slice + depth_group * 32; k0 < k_end; k0 += kFlight * kPace) {
+      uint32_t r0[kFlight][4], r1[kFlight][4], b[kFlight][RT][4];
+#pragma unroll
+      for (int f = 0; f < kFlight; f++) {
+        const uint32_t k = k0 + f * kPace;
+        const int at = (int)k + (int)c * 8, valid = k < k_end ? (int)p.dim - at : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r0[f][i] = r1[f][i] = 0;
+        if (t0 >= 0 && valid > 0) load_words<4, VECTOR>(r0[f], x + (long long)t0 * p.x_stride + at, valid);
+        if (t1 >= 0 && valid > 0) load_words<4, VECTOR>(r1[f], x + (long long)t1 * p.x_stride + at, valid);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          const uint32_t rank = rank0 + r * 8 + g;
+#pragma unroll
+          for (int i = 0; i < 4; i++) b[f][r][i] = 0;
+          if (rank < p.rank && valid > 0) load_words<4, VECTOR>(b[f][r], down + (size_t)rank * p.dim + at, valid);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; f++) {
+        const uint32_t a0[4] = {r0[f][0], r1[f][0], r0[f][1], r1[f][1]}, a1[4] = {r0[f][2], r1[f][2], r0[f][3], r1[f][3]};
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          Half<E>::mma(acc[r], a0, b[f][r][0], b[f][r][1]);
+          Half<E>::mma(acc[r], a1, b[f][r][2], b[f][r][3]);
+        }
+      }
+    }
+    float* mine = part + (size_t)depth_group * kTile * RP + rank0;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      *reinterpret_cast<float2*>(mine + g * RP + r * 8 + c * 2) = make_float2(acc[r][0], acc[r][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * RP + r * 8 + c * 2) = make_float2(acc[r][2], acc[r][3]);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x * 4; i < tile.count * RP; i += kBlock * 4) {
+      float4 sum = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll
+      for (int w = 1; w < S::kDepthGroups; w++) {
+        const float4 v = *reinterpret_cast<const float4*>(part + w * kTile * RP + i);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      *reinterpret_cast<float4*>(part + i) = sum;
+    }
+  }
+  cluster_arrive();
+  uint32_t ahead[2][4] = {};  // base of the warp's first columns
+#pragma unroll
+  for (int o = 0; o < 2; o++) {
+    const int t = token[g + 8 * o], at = (int)(n_begin + warp * 32 + c * 8), valid = (int)n_end - at;
+    if (t >= 0 && valid > 0) load_words<4, VECTOR>(ahead[o], base + (long long)t * p.base_stride + at, valid);
+  }
+  cluster_wait();
+  // the CTAs' sums, in their order; scaled to the token's largest so that both 16-bit terms keep their bits
+  {
+    const float scale = p.scale ? p.scale[tile.group] : 1.f;
+    constexpr int kRounds = (KR + 63) / 64;
+    for (uint32_t m = warp; m < kTile; m += kWarps) {
+      float2 u[kRounds];
+      float top = 0.f;
+#pragma unroll
+      for (int o = 0; o < kRounds; o++) {
+        const uint32_t r = o * 64 + lane * 2;
+        u[o] = make_float2(0.f, 0.f);
+        if (m < tile.count && r < RP) {
+          float2 v[kMostCluster];
+#pragma unroll
+          for (int w = 0; w < kMostCluster; w++)
+            if (w < members) v[w] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(part, w) + m * RP + r);
+#pragma unroll
+          for (int w = 0; w < kMostCluster; w++)
+            if (w < members) u[o].x += v[w].x, u[o].y += v[w].y;
+          u[o].x *= scale, u[o].y *= scale;
+        }
+        top = fmaxf(top, fmaxf(fabsf(u[o].x), fabsf(u[o].y)));
+      }
+#pragma unroll
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+      const float s = unit_scale(top);
+      if (lane == 0) back[m] = 1.f / s;
+#pragma unroll
+      for (int o = 0; o < kRounds; o++) {
+        const uint32_t r = o * 64 + lane * 2;
+        if (r >= KR) continue;
+        const float u0 = u[o].x * s, u1 = u[o].y * s;
+        const uint32_t hi = Half<E>::narrow(u0, u1);
+        const float2 h = Half<E>::widen(hi);
+        // what the first term leaves; nothing where the first is infinite
+        const uint32_t lo = Half<E>::narrow(isinf(h.x) ? 0.f : u0 - h.x, isinf(h.y) ? 0.f : u1 - h.y);
+        *reinterpret_cast<uint32_t*>(&inner[0][m][r]) = hi;
+        *reinterpret_cast<uint32_t*>(&inner[1][m][r]) = lo;
+      }
+    }
+  }
+  __syncthreads();
+  cluster_arrive();  // waited for at the end: nobody leaves while its sums are being read
+  if (held) barrier_wait(shared_address(&up_landed), 0);
+
+  // second product: every CTA a slice of out_dim, 32 of it a warp at a time.  Column 2c + b of the
+  // q-th of four matrix tiles is output 8c + 2q + b, so that a lane ends with 8 consecutive outputs.
+  {
+    constexpr int KS = KR >= 32 ? KR / 32 : 1;   // steps of 32 (16) ranks
+    constexpr int W = KR >= 32 ? 4 : 2;          // words a lane has of one
+    uint32_t u[2][2][KS][W];                     // term, half of the tile
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int o = 0; o < 2; o++)
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+          load_words<W, true>(u[h][o][s], &inner[h][g + 8 * o][(s * 4 + c) * 2 * W], 2 * W);
+    for (uint32_t n0 = n_begin + warp * 32; n0 < n_end; n0 += kWarps * 32) {
+      const int at = (int)(n0 + c * 8), valid = (int)n_end - at;
+      uint32_t in[2][4];
+#pragma unroll
+      for (int o = 0; o < 2; o++) {
+        const int t = token[g + 8 * o];
+#pragma unroll
+        for (int i = 0; i < 4; i++) in[o][i] = ahead[o][i];
+        if (n0 != n_begin + warp * 32 && t >= 0 && valid > 0) load_words<4, VECTOR>(in[o], base + (long long)t * p.base_stride + at, valid);
+      }
+      float acc[4][4] = {};
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const uint32_t n = n0 + (g >> 1) * 8 + q * 2 + (g & 1);
+        const uint16_t* row = n - n_begin < held ? up_here + (size_t)(n - n_begin) * p.rank : up + (size_t)n * p.rank;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+          uint32_t b[W] = {};
+          const int r = (s * 4 + (int)c) * 2 * W, left = (int)p.rank - r;
+          if (n < n_end && left > 0) load_words<W, VECTOR>(b, row + r, left);
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int w = 0; w < W; w += 2) {
+              const uint32_t a[4] = {u[h][0][s][w], u[h][1][s][w], u[h][0][s][w + 1], u[h][1][s][w + 1]};
+              Half<E>::mma(acc[q], a, b[w], b[w + 1]);
+            }
+        }
+      }
+#pragma unroll
+      for (int o = 0; o < 2; o++) {
+        const int t = token[g + 8 * o];
+        if (t < 0 || valid <= 0) continue;
+        const float s = back[g + 8 * o];
+        uint32_t y[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const float2 v = Half<E>::widen(in[o][q]);
+          y[q] = Half<E>::narrow(fmaf(acc[q][2 * o], s, v.x), fmaf(acc[q][2 * o + 1], s, v.y));
+        }
+        uint16_t* to = out + (long long)t * p.out_stride + at;
+        if (VECTOR && valid >= 8) {
+          *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (i < valid) to[i] = (uint16_t)(y[i / 2] >> (i & 1 ? 16 : 0));
+        }
+      }
+    }
+  }
+  cluster_wait();
+}
+
+// ------------------------------------------------------------------------------------
+// prompts: tiles of 128 tokens on the 5th-generation tensor cores
+// ------------------------------------------------------------------------------------
+// Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
+// partial sums in the workspace; the second adds those up, splits them into two 16-bit terms and multiplies
+// them with `up`, adding `base` on the way out.  In both a tile is so many steps of 64 columns, the tiles of the
+// batch stand one behind the other, and every CTA of a full GPU takes the same number of consecutive
+// steps, so that no number of tiles leaves part of the GPU idle; where a CTA's run starts or ends inside a tile
+// of the first product, the tile has one more partial sum.
+// Steps go through a ring of stages in shared memory: four warps copy (token rows lie anywhere, so 16
+// bytes a thread), one thread issues the matrix instructions, the other warps take the products out of
+// tensor memory.
+//
+// Operands lie in shared memory in rows of 128 bytes whose 16-byte pieces are exchanged by row (piece c
+// of row r at c ^ (r % 8)), as the matrix unit reads them: a line of global memory is a line there, and
+// one token a thread reads `base` without bank conflicts.  (Blocks of 8 rows x 16 bytes, the other layout
+// the unit takes, split every line over eight and cost 2.5 times the time.)
+
+constexpr int kBigTile = 128;
+constexpr int kStep = 128;                                  // columns a step
+constexpr int kBlock64 = kBigTile * 128;                    // 64 columns of a tile's rows
+constexpr int kRowsBytes = kBigTile * kStep * 2;            // x or base of a step
+constexpr int kProducers = 128;
+constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, multiply
+constexpr int kUpThreads = kProducers + 256 + 32;
+constexpr int kMostTiles = 36;                              // a CTA's run touches
+
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
@@ -855,34 +948,46 @@ __global__ void __launch_bounds__(kUpThreads, 1)
 template <typename E, int RP>
 cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t stream) {
   auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
-  constexpr size_t smem = kWarps * kTile * RP * sizeof(float) + 2 * kTile * (std::max(RP, 16) + 8) * sizeof(uint16_t);
-  if (smem > 47 * 1024) {  // beside what is static
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+  using S = SmallShape<RP>;
+  constexpr uint32_t kSms = 148, kMostPerSm = RP <= 16 ? 4 : RP <= 32 ? 3 : 2;  // by registers
   const uint32_t tiles = p.n_tokens / kTile + std::min(p.n_groups + 1, p.n_tokens);
+  // clusters of 8 are the shorter chain, of 4 the less work a tile: they win from one and a half waves on
+  const uint32_t cluster = tiles * kMostCluster > kSms * kMostPerSm * 3 / 2 ? kMostCluster / 2 : kMostCluster;
+  // Few CTAs take as much shared memory as spreads them over all SMs (packed onto few of them, 30 tiles of rank 16 took
+  // 9.8 us instead of 8.4); what is left of it holds `up`.
+  const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, kMostPerSm);
+  const uint32_t budget = std::min(216u * 1024 / per_sm, 200u * 1024);
+  const uint32_t slice = (p.out_dim + cluster * 32 - 1) / (cluster * 32) * 32;
+  const uint32_t room = vector ? (uint32_t)std::min<size_t>(budget - S::kShared, (size_t)slice * p.rank * 2) / 16 * 16 : 0;
+  const size_t smem = budget;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * kCluster);
+  cfg.gridDim = dim3(tiles * cluster);
   cfg.blockDim = dim3(kBlock);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {kCluster, 1, 1};
+  attr[0].val.clusterDim = {cluster, 1, 1};
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  return cudaLaunchKernelEx(&cfg, kern, p, room);
 }
+
+int padded_rank(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 // Runs of both products.  At most: every group may end in a tile of its own.
 struct BigSplit {
   BigShare down, up;
   uint32_t parts;  // partial sums a tile has, at most
 };
-BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t dim, uint32_t out_dim) {
-  constexpr uint32_t kSlots = 148, kMostParts = 8, kLeastUp = 2;
+BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t dim, uint32_t out_dim) {
+  constexpr uint32_t kSlots = 148, kLeastUp = 2;
+  // what a run of the second product reads first is 512 bytes x ranks x parts
+  const uint32_t most_parts = std::max(3, std::min(8, 256 / padded_rank(rank)));
   const uint32_t most_tiles = n_tokens / kBigTile + std::min(n_groups + 1, n_tokens), tiles = (n_tokens + kBigTile - 1) / kBigTile;
   const uint32_t grid = std::max(kSlots, (most_tiles + kMostTiles - 4) / (kMostTiles - 3));
   auto over = [](unsigned long long a, unsigned long long b) { return (uint32_t)((a + b - 1) / b); };
@@ -890,14 +995,20 @@ BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t dim, uint32_t 
   b.down.tile_steps = over(dim, kStep);
   b.up.tile_steps = over(out_dim, kStep);
   b.down.grid = b.up.grid = grid;
-  b.down.least = std::max(over((unsigned long long)tiles * b.down.tile_steps, grid), over(b.down.tile_steps, kMostParts - 1));
+  b.down.least = std::max(over((unsigned long long)tiles * b.down.tile_steps, grid), over(b.down.tile_steps, most_parts - 1));
   b.up.least = std::min(kLeastUp, b.up.tile_steps);
   b.parts = over(b.down.tile_steps, b.down.least) + 1;
   return b;
 }
-int padded_rank(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
-bool big_batch(uint32_t n_tokens, uint32_t n_groups) { return n_tokens >= 512 && n_tokens >= 16 * n_groups; }
+// Tiles of 128 or of 16 tokens.  Against a tile of 16, one of 128 reads an adapter's matrices an eighth as often
+// but has a longer chain and two launches; what the former costs grows with tokens x rank.  Measured, 4096 x 4096, 16 | 128 a tile, us:
+// rank 16: 2048 tokens of 8 adapters 20.9 | 22.4, 4096 of 8 39.7 | 27.5, 4096 of 128 50 | 48, 4096 of 256 46 | 57;
+// rank 64: 256 of 8 14 | 19, 1024 of 32 46 | 30, 1024 of 64 47 | 29; rank 128: 256 of 8 24 | 29, 512 of 8 44 | 34.
+bool big_batch(uint32_t n_tokens, uint32_t n_groups, uint32_t rank) {
+  const unsigned long long work = (unsigned long long)n_tokens * padded_rank(rank);
+  return work >= 40960 && work >= 512ull * n_groups;
+}
 
 template <typename E, int RP>
 cudaError_t big_launch(const AdapterParams& p, float* inner, cudaStream_t stream) {
@@ -907,7 +1018,7 @@ cudaError_t big_launch(const AdapterParams& p, float* inner, cudaStream_t stream
   cudaError_t e = cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kDownShared);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kUpShared);
   if (e != cudaSuccess) return e;
-  const BigSplit b = big_split(p.n_tokens, p.n_groups, p.dim, p.out_dim);
+  const BigSplit b = big_split(p.n_tokens, p.n_groups, p.rank, p.dim, p.out_dim);
   cudaLaunchConfig_t cfg = {};
   cfg.stream = stream;
   cudaLaunchAttribute attr = {};
@@ -929,8 +1040,8 @@ cudaError_t big_launch(const AdapterParams& p, float* inner, cudaStream_t stream
 }  // namespace
 
 size_t adapter_scratch_bytes(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t dim, uint32_t out_dim) {
-  if (!big_batch(n_tokens, n_groups)) return 0;
-  return (size_t)big_split(n_tokens, n_groups, dim, out_dim).parts * n_tokens * padded_rank(rank) * sizeof(float);
+  if (!big_batch(n_tokens, n_groups, rank)) return 0;
+  return (size_t)big_split(n_tokens, n_groups, rank, dim, out_dim).parts * n_tokens * padded_rank(rank) * sizeof(float);
 }
 
 cudaError_t adapter_stalled(uint32_t* count) { return cudaMemcpyFromSymbol(count, g_stalled, sizeof(*count)); }
@@ -944,7 +1055,7 @@ cudaError_t launch_adapter_add(const AdapterParams& p, int elem, void* scratch, 
   const bool vector = addresses % 16 == 0 && strides % 8 == 0 && p.dim % 8 == 0 && p.out_dim % 8 == 0 && p.rank % 8 == 0;
   auto by_rank = [&](auto e) {
     using E = decltype(e);
-    if (vector && big_batch(p.n_tokens, p.n_groups)) {
+    if (vector && big_batch(p.n_tokens, p.n_groups, p.rank)) {
       float* inner = static_cast<float*>(scratch);
       switch (padded_rank(p.rank)) {
         case 16: return big_launch<E, 16>(p, inner, stream);
