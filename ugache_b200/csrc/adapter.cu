@@ -166,6 +166,33 @@ constexpr int kMostCluster = 8;
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// Columns [begin, end) of the tokens' rows from one matrix to another; by the whole CTA, four pieces a thread in flight.
+template <int ROWS, bool VECTOR>
+__device__ __forceinline__ void copy_rows(const uint16_t* from, long long from_stride, uint16_t* to, long long to_stride,
+                                          const int32_t* token, uint32_t count, uint32_t begin, uint32_t end) {
+  constexpr uint32_t kPiece = VECTOR ? 8 : 1;
+  const uint32_t pieces = (end - begin + kPiece - 1) / kPiece, all = count * pieces;
+  for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 4 * kBlock) {
+    uint4 v[4];
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+      const uint32_t i = i0 + f * kBlock, m = i / pieces, n = begin + i % pieces * kPiece;
+      if (i >= all || token[m] < 0) continue;
+      const uint16_t* at = from + (long long)token[m] * from_stride + n;
+      if (VECTOR) v[f] = *reinterpret_cast<const uint4*>(at);
+      else v[f].x = *at;
+    }
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+      const uint32_t i = i0 + f * kBlock, m = i / pieces, n = begin + i % pieces * kPiece;
+      if (i >= all || token[m] < 0) continue;
+      uint16_t* at = to + (long long)token[m] * to_stride + n;
+      if (VECTOR) *reinterpret_cast<uint4*>(at) = v[f];
+      else *at = (uint16_t)v[f].x;
+    }
+  }
+}
+
 // RP: rank rounded up to 8, 16, 32, 64 or 128.
 template <int RP>
 struct SmallShape {
@@ -179,7 +206,7 @@ struct SmallShape {
 };
 
 template <typename E, int RP, bool VECTOR>
-__global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32_t up_room) {
+__global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapter_kernel(AdapterParams p, uint32_t up_room) {
   using S = SmallShape<RP>;
   constexpr int KR = S::kDepth;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -227,21 +254,9 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32
 
   if (bare) {  // no adapter
     if (out == base) return;
-    for (uint32_t m = warp; m < tile.count; m += kWarps) {
-      if (token[m] < 0) continue;
-      const uint16_t* from = base + (long long)token[m] * p.base_stride;
-      uint16_t* to = out + (long long)token[m] * p.out_stride;
-      for (uint32_t n = n_begin + lane * 8; n < n_end; n += 256) {
-        if (VECTOR && n + 8 <= n_end) {
-          *reinterpret_cast<uint4*>(to + n) = *reinterpret_cast<const uint4*>(from + n);
-        } else {
-          for (uint32_t i = n; i < min(n + 8, n_end); i++) to[i] = from[i];
-        }
-      }
-    }
+    copy_rows<kTile, VECTOR>(base, p.base_stride, out, p.out_stride, token, tile.count, n_begin, n_end);
     return;
   }
-
   // first product: every CTA a slice of dim, 32 of it a warp at a time, several such loads in flight
   {
     const uint16_t* down = static_cast<const uint16_t*>(p.down) + (long long)tile.group * p.down_stride;
@@ -299,12 +314,15 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32
     }
   }
   cluster_arrive();
-  uint32_t ahead[2][4] = {};  // base of the warp's first columns
+  uint32_t in[2][4] = {};  // base of the warp's next columns
+  auto load_base = [&](uint32_t n0) {
 #pragma unroll
-  for (int o = 0; o < 2; o++) {
-    const int t = token[g + 8 * o], at = (int)(n_begin + warp * 32 + c * 8), valid = (int)n_end - at;
-    if (t >= 0 && valid > 0) load_words<4, VECTOR>(ahead[o], base + (long long)t * p.base_stride + at, valid);
-  }
+    for (int o = 0; o < 2; o++) {
+      const int t = token[g + 8 * o], at = (int)(n0 + c * 8), valid = (int)n_end - at;
+      if (t >= 0 && valid > 0) load_words<4, VECTOR>(in[o], base + (long long)t * p.base_stride + at, valid);
+    }
+  };
+  load_base(n_begin + warp * 32);
   cluster_wait();
   // the CTAs' sums, in their order; scaled to the token's largest so that both 16-bit terms keep their bits
   {
@@ -366,14 +384,12 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32
           load_words<W, true>(u[h][o][s], &inner[h][g + 8 * o][(s * 4 + c) * 2 * W], 2 * W);
     for (uint32_t n0 = n_begin + warp * 32; n0 < n_end; n0 += kWarps * 32) {
       const int at = (int)(n0 + c * 8), valid = (int)n_end - at;
-      uint32_t in[2][4];
+      uint32_t y[2][4];
 #pragma unroll
-      for (int o = 0; o < 2; o++) {
-        const int t = token[g + 8 * o];
+      for (int o = 0; o < 2; o++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) in[o][i] = ahead[o][i];
-        if (n0 != n_begin + warp * 32 && t >= 0 && valid > 0) load_words<4, VECTOR>(in[o], base + (long long)t * p.base_stride + at, valid);
-      }
+        for (int i = 0; i < 4; i++) y[o][i] = in[o][i];
+      load_base(n0 + kWarps * 32);
       float acc[4][4] = {};
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -398,19 +414,18 @@ __global__ void __launch_bounds__(kBlock) adapter_kernel(AdapterParams p, uint32
         const int t = token[g + 8 * o];
         if (t < 0 || valid <= 0) continue;
         const float s = back[g + 8 * o];
-        uint32_t y[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-          const float2 v = Half<E>::widen(in[o][q]);
-          y[q] = Half<E>::narrow(fmaf(acc[q][2 * o], s, v.x), fmaf(acc[q][2 * o + 1], s, v.y));
+          const float2 v = Half<E>::widen(y[o][q]);
+          y[o][q] = Half<E>::narrow(fmaf(acc[q][2 * o], s, v.x), fmaf(acc[q][2 * o + 1], s, v.y));
         }
         uint16_t* to = out + (long long)t * p.out_stride + at;
         if (VECTOR && valid >= 8) {
-          *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(to) = make_uint4(y[o][0], y[o][1], y[o][2], y[o][3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; i++)
-            if (i < valid) to[i] = (uint16_t)(y[i / 2] >> (i & 1 ? 16 : 0));
+            if (i < valid) to[i] = (uint16_t)(y[o][i / 2] >> (i & 1 ? 16 : 0));
         }
       }
     }
@@ -947,15 +962,19 @@ __global__ void __launch_bounds__(kUpThreads, 1)
 
 template <typename E, int RP>
 cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t stream) {
-  auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
   using S = SmallShape<RP>;
-  constexpr uint32_t kSms = 148, kMostPerSm = RP <= 16 ? 4 : RP <= 32 ? 3 : 2;  // by registers
+  auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
+  constexpr uint32_t kSms = 148;
   const uint32_t tiles = p.n_tokens / kTile + std::min(p.n_groups + 1, p.n_tokens);
-  // clusters of 8 are the shorter chain, of 4 the less work a tile: they win from one and a half waves on
-  const uint32_t cluster = tiles * kMostCluster > kSms * kMostPerSm * 3 / 2 ? kMostCluster / 2 : kMostCluster;
-  // Few CTAs take as much shared memory as spreads them over all SMs (packed onto few of them, 30 tiles of rank 16 took
-  // 9.8 us instead of 8.4); what is left of it holds `up`.
-  const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, kMostPerSm);
+  // Clusters of 8 are the shorter chain, of 4 the less work a tile: 64 tiles of rank 16 (4096 x 4096) 10.7 against 13.3 us,
+  // 128 tiles 15.6 against 12.8.
+  const bool few = tiles * kMostCluster <= kSms * 9 / 2;
+  const uint32_t cluster = few ? kMostCluster : kMostCluster / 2;
+  // CTAs an SM, by shared memory: as few as hold the batch, so that they spread over all SMs (packed onto few
+  // of them 30 tiles took 9.9 us instead of 8.5), and of small clusters at most three (mixed prompts of 200 adapters 18.7 us
+  // with four, 16.4 with three).  What is left of it holds `up`.
+  constexpr uint32_t kMost = RP <= 32 ? 3 : 2;
+  const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, few && RP <= 16 ? 4 : kMost);
   const uint32_t budget = std::min(216u * 1024 / per_sm, 200u * 1024);
   const uint32_t slice = (p.out_dim + cluster * 32 - 1) / (cluster * 32) * 32;
   const uint32_t room = vector ? (uint32_t)std::min<size_t>(budget - S::kShared, (size_t)slice * p.rank * 2) / 16 * 16 : 0;
