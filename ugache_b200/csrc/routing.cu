@@ -223,19 +223,9 @@ void plan_parts(uint32_t n, uint32_t* parts, uint32_t* part) {
 // rows
 // ------------------------------------------------------------------------------------
 
-template <int BYTES>
-struct Piece;
-template <>
-struct __align__(16) Piece<16> {
+// Rows move in pieces of 16 bytes.
+struct __align__(16) Piece {
   uint32_t v[4];
-};
-template <>
-struct __align__(4) Piece<4> {
-  uint32_t v[1];
-};
-template <>
-struct __align__(2) Piece<2> {
-  uint16_t v[1];
 };
 
 template <typename E>
@@ -255,191 +245,422 @@ __device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
 
-template <typename E, int BYTES>
+template <typename E>
 struct Floats {
-  static constexpr int N = BYTES / (int)sizeof(E);
+  static constexpr int N = 16 / (int)sizeof(E);
   float f[N];
-  __device__ __forceinline__ void from(const Piece<BYTES>& p) {
+  __device__ __forceinline__ void from(const Piece& p) {
     const E* e = reinterpret_cast<const E*>(&p);
 #pragma unroll
     for (int i = 0; i < N; i++) f[i] = widen<E>(e[i]);
   }
-  __device__ __forceinline__ Piece<BYTES> rounded() const {
-    Piece<BYTES> p;
+  // The sums were fp32; this is their one rounding.
+  __device__ __forceinline__ Piece rounded() const {
+    Piece p;
     E* e = reinterpret_cast<E*>(&p);
 #pragma unroll
     for (int i = 0; i < N; i++) e[i] = narrow<E>(f[i]);
     return p;
   }
+  __device__ __forceinline__ void add(const Floats& x) {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] += x.f[i];
+  }
+  __device__ __forceinline__ void add(const Floats& x, float w) {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = fmaf(w, x.f[i], f[i]);
+  }
+  __device__ __forceinline__ Floats times(float w) const {
+    Floats y;
+#pragma unroll
+    for (int i = 0; i < N; i++) y.f[i] = w * f[i];
+    return y;
+  }
+  __device__ __forceinline__ float dot(const Floats& x, float sum) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) sum = fmaf(f[i], x.f[i], sum);
+    return sum;
+  }
 };
 
-template <int BYTES>
-__device__ __forceinline__ Piece<BYTES> ld_piece(const void* base, long long stride, uint32_t row, uint32_t piece) {
-  return *reinterpret_cast<const Piece<BYTES>*>(static_cast<const char*>(base) + (long long)row * stride + (size_t)piece * BYTES);
+__device__ __forceinline__ const char* row_at(const void* base, long long stride, uint32_t row) {
+  return static_cast<const char*>(base) + (long long)row * stride;
 }
-template <int BYTES>
-__device__ __forceinline__ void st_piece(void* base, long long stride, uint32_t row, uint32_t piece, const Piece<BYTES>& p) {
-  *reinterpret_cast<Piece<BYTES>*>(static_cast<char*>(base) + (long long)row * stride + (size_t)piece * BYTES) = p;
+__device__ __forceinline__ char* row_at(void* base, long long stride, uint32_t row) {
+  return static_cast<char*>(base) + (long long)row * stride;
+}
+__device__ __forceinline__ Piece ld_piece(const char* row, uint32_t piece) {
+  return *reinterpret_cast<const Piece*>(row + (size_t)piece * 16);
+}
+__device__ __forceinline__ void st_piece(char* row, uint32_t piece, const Piece& p) {
+  *reinterpret_cast<Piece*>(row + (size_t)piece * 16) = p;
 }
 
-// Rows of row_out that no choice took.
-template <int BYTES>
-__device__ __forceinline__ void zero_tail(const RouteRows& p, uint32_t pieces) {
-  if (!p.n_routed) return;
-  const uint32_t routed = min((uint32_t)max(*p.n_routed, 0), p.n_rows);
-  const Piece<BYTES> zero = {};
-  const unsigned long long n = (unsigned long long)(p.n_rows - routed) * pieces;
-  for (unsigned long long u = (unsigned long long)blockIdx.x * blockDim.x + threadIdx.x; u < n;
-       u += (unsigned long long)gridDim.x * blockDim.x)
-    st_piece<BYTES>(p.row_out, p.row_out_stride, routed + (uint32_t)(u / pieces), (uint32_t)(u % pieces), zero);
+// Place of a choice among the rows; kNowhere where it has none.
+constexpr uint32_t kNowhere = 0xffffffffu;
+__device__ __forceinline__ uint32_t place_of(const RouteRows& p, size_t choice) {
+  const uint32_t row = (uint32_t)p.position[choice];
+  return row < p.n_rows ? row : kNowhere;
+}
+// First row of row_out that no choice took, n_rows if they are not to be zeroed.
+__device__ __forceinline__ uint32_t first_untaken(const RouteRows& p) {
+  return p.n_routed ? min((uint32_t)max(*p.n_routed, 0), p.n_rows) : p.n_rows;
+}
+
+// n / d of a thread's number in the launch; 64-bit division is several times the instructions
+__device__ __forceinline__ void divide(unsigned long long n, uint32_t d, uint32_t* q, uint32_t* r) {
+  if (n >> 32 == 0) {
+    *q = (uint32_t)n / d;
+    *r = (uint32_t)n - *q * d;
+  } else {
+    *q = (uint32_t)(n / d);
+    *r = (uint32_t)(n - (unsigned long long)*q * d);
+  }
 }
 
 constexpr int kRowsBlock = 256;
 
-// A thread has one piece of one token's row and takes it to all the rows of the token's choices.
-template <typename E, int BYTES, bool WEIGHTED>
+__device__ __forceinline__ void zero_untaken(const RouteRows& p, uint32_t pieces) {
+  const uint32_t first = first_untaken(p);
+  const unsigned long long n = (unsigned long long)(p.n_rows - first) * pieces;
+  for (unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x; u < n;
+       u += (unsigned long long)gridDim.x * kRowsBlock) {
+    uint32_t row, c;
+    divide(u, pieces, &row, &c);
+    st_piece(row_at(p.row_out, p.row_out_stride, first + row), c, Piece{});
+  }
+}
+
+// A thread has one piece of one token's row and takes it to the rows of the token's choices.  Bound by the
+// writes: 16,384 tokens of 4 KiB to 8 rows each 96 us, 6.3 TB/s.
+template <typename E, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowsBlock) spread_kernel(RouteRows p, uint32_t pieces) {
   wait_for_launch_ahead();
   release_launch_behind();
-  const unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x;
-  const uint32_t t = (uint32_t)(u / pieces), c = (uint32_t)(u % pieces);
+  uint32_t t, c;
+  divide((unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x, pieces, &t, &c);
   if (t < p.n_tokens) {
-    const Piece<BYTES> in = ld_piece<BYTES>(p.token_in, p.token_in_stride, t, c);
-    Floats<E, BYTES> x;
+    const Piece in = ld_piece(row_at(p.token_in, p.token_in_stride, t), c);
+    Floats<E> x;
     if (WEIGHTED) x.from(in);
     const size_t at = (size_t)t * p.k;
     for (uint32_t j = 0; j < p.k; j++) {
-      const uint32_t row = (uint32_t)p.position[at + j];
-      if (row >= p.n_rows) continue;
-      if (WEIGHTED) {
-        const float w = p.weights[at + j];
-        Floats<E, BYTES> y;
-#pragma unroll
-        for (int i = 0; i < x.N; i++) y.f[i] = w * x.f[i];
-        st_piece<BYTES>(p.row_out, p.row_out_stride, row, c, y.rounded());
-      } else {
-        st_piece<BYTES>(p.row_out, p.row_out_stride, row, c, in);
-      }
+      const uint32_t row = place_of(p, at + j);
+      if (row == kNowhere) continue;
+      st_piece(row_at(p.row_out, p.row_out_stride, row), c, WEIGHTED ? x.times(p.weights[at + j]).rounded() : in);
     }
   }
-  zero_tail<BYTES>(p, pieces);
+  zero_untaken(p, pieces);
 }
 
-// A thread sums one piece of one token's row over its choices, in their order, in fp32.
-template <typename E, int BYTES, bool WEIGHTED>
+// A thread sums PIECES pieces of one token's row over its choices, in their order, in fp32: FLIGHT choices and
+// all pieces are on their way at once.
+template <typename E, bool WEIGHTED, int FLIGHT, int PIECES>
 __global__ void __launch_bounds__(kRowsBlock) gather_kernel(RouteRows p, uint32_t pieces) {
   wait_for_launch_ahead();
   release_launch_behind();
-  const unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x;
-  const uint32_t t = (uint32_t)(u / pieces), c = (uint32_t)(u % pieces);
+  const uint32_t stride = pieces / PIECES;  // between a thread's pieces
+  uint32_t t, c;
+  divide((unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x, stride, &t, &c);
   if (t >= p.n_tokens) return;
-  constexpr int kFlight = 4;
   const size_t at = (size_t)t * p.k;
-  Floats<E, BYTES> sum = {};
-  for (uint32_t j0 = 0; j0 < p.k; j0 += kFlight) {
-    uint32_t row[kFlight];
-    float w[kFlight];
-    Piece<BYTES> in[kFlight];
+  Floats<E> sum[PIECES] = {};
+  for (uint32_t j0 = 0; j0 < p.k; j0 += FLIGHT) {
+    uint32_t row[FLIGHT];
+    float w[FLIGHT];
+    Piece in[FLIGHT][PIECES];
 #pragma unroll
-    for (int j = 0; j < kFlight; j++) {
-      row[j] = j0 + j < p.k ? (uint32_t)p.position[at + j0 + j] : kFull;
-      if (row[j] < p.n_rows) {
-        in[j] = ld_piece<BYTES>(p.row_in, p.row_in_stride, row[j], c);
-        if (WEIGHTED) w[j] = p.weights[at + j0 + j];
+    for (int j = 0; j < FLIGHT; j++) {
+      row[j] = j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
+      w[j] = WEIGHTED && row[j] != kNowhere ? p.weights[at + j0 + j] : 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < FLIGHT; j++)
+      if (row[j] != kNowhere) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) in[j][i] = ld_piece(row_at(p.row_in, p.row_in_stride, row[j]), c + i * stride);
       }
-    }
 #pragma unroll
-    for (int j = 0; j < kFlight; j++) {
-      if (row[j] >= p.n_rows) continue;
-      Floats<E, BYTES> x;
-      x.from(in[j]);
+    for (int j = 0; j < FLIGHT; j++)
+      if (row[j] != kNowhere) {
 #pragma unroll
-      for (int i = 0; i < x.N; i++) sum.f[i] = WEIGHTED ? fmaf(w[j], x.f[i], sum.f[i]) : sum.f[i] + x.f[i];
-    }
+        for (int i = 0; i < PIECES; i++) {
+          Floats<E> x;
+          x.from(in[j][i]);
+          if (WEIGHTED) sum[i].add(x, w[j]);
+          else sum[i].add(x);
+        }
+      }
   }
-  st_piece<BYTES>(p.token_out, p.token_out_stride, t, c, sum.rounded());
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) st_piece(row_at(p.token_out, p.token_out_stride, t), c + i * stride, sum[i].rounded());
 }
 
-// With inner products: `group` threads (a power of two) have one token; they walk its row together,
-// a lane sums its share of each choice's product in fp32, the shares are added in a fixed order.
-constexpr int kDots = 8;  // choices a pass
+// The sums of N (a power of two) values of each lane over `width` lanes: at every step a lane keeps half of its
+// values and hands over the others, so that it takes N - 1 + log2(width / N) exchanges instead of N * log2(width).  The
+// order of the additions is the same wherever a value ends.  Returns the sum of value `which`.
+template <int N>
+__device__ __forceinline__ float sum_over_warp(float (&v)[N], uint32_t* which) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t at = 0;
+  int n = N, d = 16;
+#pragma unroll
+  for (int step = N; step > 1; step >>= 1, d >>= 1) {
+    n = step / 2;
+    const bool upper = lane & d;
+#pragma unroll
+    for (int i = 0; i < N / 2; i++)
+      if (i < n) {
+        const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+        v[i] = keep + __shfl_xor_sync(kFull, give, d);
+      }
+    if (upper) at += n;
+  }
+#pragma unroll
+  for (; d; d >>= 1) v[0] += __shfl_xor_sync(kFull, v[0], d);
+  *which = at;
+  return v[0];
+}
 
-template <typename E, int BYTES, bool WEIGHTED, bool SPREAD>
-__global__ void __launch_bounds__(kRowsBlock) dots_kernel(RouteRows p, uint32_t pieces, uint32_t group) {
+// The lanes' sums of N choices' products into the dots: by the whole CTA.
+template <int N>
+__device__ __forceinline__ void share_sums(float (&dot)[N], float (*share)[N], const RouteRows& p, size_t at, uint32_t j0,
+                                           bool live, uint32_t lane, uint32_t lanes) {
+  if (lanes < 32) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      for (uint32_t d = lanes >> 1; d; d >>= 1) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
+      if (live && lane == 0 && j0 + j < p.k) p.dots[at + j0 + j] = dot[j];
+    }
+    return;
+  }
+  uint32_t which;
+  const float sum = sum_over_warp(dot, &which);
+  const bool has = (lane & (32 / N - 1)) == 0;  // one lane of those that end with the value
+  if (lanes == 32) {
+    if (has && live && j0 + which < p.k) p.dots[at + j0 + which] = sum;
+    return;
+  }
+  __syncthreads();
+  if (has) share[threadIdx.x >> 5][which] = sum;
+  __syncthreads();
+  if (lane < N && live && j0 + lane < p.k) {
+    float all = 0.f;
+    for (uint32_t i = 0; i < lanes / 32; i++) all += share[(threadIdx.x >> 5) + i][lane];
+    p.dots[at + j0 + lane] = all;
+  }
+}
+
+// Inner products of a token's row with the rows of its choices, and the spread or the gather on the way: `lanes`
+// threads (a power of two, fixed by the row's length, so that results do not depend on the batch) walk the row
+// together.  All rows' pieces are loaded before anything is stored.
+template <typename E, bool WEIGHTED, bool SPREAD, int CHOICES>
+__global__ void __launch_bounds__(kRowsBlock, 2) dots_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
   wait_for_launch_ahead();
   release_launch_behind();
-  __shared__ float share[kRowsBlock / 32][kDots];
-  const uint32_t in_group = threadIdx.x & (group - 1);
-  const uint32_t t = blockIdx.x * (kRowsBlock / group) + threadIdx.x / group;
+  __shared__ float share[kRowsBlock / 32][CHOICES];
+  const uint32_t lane = threadIdx.x & (lanes - 1);
+  const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
   const bool live = t < p.n_tokens;
   const size_t at = (size_t)t * p.k;
-  for (uint32_t j0 = 0; j0 < p.k; j0 += kDots) {
-    uint32_t row[kDots];
-    float w[kDots], dot[kDots];
+  for (uint32_t j0 = 0; j0 < p.k; j0 += CHOICES) {
+    uint32_t row[CHOICES];
+    float w[CHOICES], dot[CHOICES];
 #pragma unroll
-    for (int j = 0; j < kDots; j++) {
+    for (int j = 0; j < CHOICES; j++) {
       dot[j] = 0.f;
-      row[j] = live && j0 + j < p.k ? (uint32_t)p.position[at + j0 + j] : kFull;
-      w[j] = WEIGHTED && row[j] < p.n_rows ? p.weights[at + j0 + j] : 1.f;
+      row[j] = live && j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
+      w[j] = WEIGHTED && row[j] != kNowhere ? p.weights[at + j0 + j] : 1.f;
     }
-    for (uint32_t c = in_group; live && c < pieces; c += group) {
-      Floats<E, BYTES> x, y;
-      x.from(ld_piece<BYTES>(p.token_in, p.token_in_stride, t, c));
-      Floats<E, BYTES> sum = {};
+    for (uint32_t c = lane; live && c < pieces; c += lanes) {
+      Piece in[CHOICES];
+      const Piece mine = ld_piece(row_at(p.token_in, p.token_in_stride, t), c);
 #pragma unroll
-      for (int j = 0; j < kDots; j++) {
-        if (row[j] >= p.n_rows) continue;
-        y.from(ld_piece<BYTES>(p.row_in, p.row_in_stride, row[j], c));
+      for (int j = 0; j < CHOICES; j++)
+        if (row[j] != kNowhere) in[j] = ld_piece(row_at(p.row_in, p.row_in_stride, row[j]), c);
+      Floats<E> x, y, sum = {};
+      x.from(mine);
 #pragma unroll
-        for (int i = 0; i < x.N; i++) {
-          dot[j] = fmaf(x.f[i], y.f[i], dot[j]);
-          if (!SPREAD) sum.f[i] = WEIGHTED ? fmaf(w[j], y.f[i], sum.f[i]) : sum.f[i] + y.f[i];
+      for (int j = 0; j < CHOICES; j++)
+        if (row[j] != kNowhere) {
+          y.from(in[j]);
+          dot[j] = x.dot(y, dot[j]);
+          if (SPREAD) {
+            st_piece(row_at(p.row_out, p.row_out_stride, row[j]), c, WEIGHTED ? x.times(w[j]).rounded() : mine);
+          } else if (WEIGHTED) {
+            sum.add(y, w[j]);
+          } else {
+            sum.add(y);
+          }
         }
-        if (SPREAD) {
-#pragma unroll
-          for (int i = 0; i < x.N; i++) y.f[i] = WEIGHTED ? w[j] * x.f[i] : x.f[i];
-          st_piece<BYTES>(p.row_out, p.row_out_stride, row[j], c, y.rounded());
-        }
-      }
       if (!SPREAD && j0 == 0) {  // choices past the first pass join the sum here, their products come later
-        for (uint32_t j = kDots; j < p.k; j++) {
-          const uint32_t r = (uint32_t)p.position[at + j];
-          if (r >= p.n_rows) continue;
-          const float v = WEIGHTED ? p.weights[at + j] : 1.f;
-          y.from(ld_piece<BYTES>(p.row_in, p.row_in_stride, r, c));
-#pragma unroll
-          for (int i = 0; i < x.N; i++) sum.f[i] = WEIGHTED ? fmaf(v, y.f[i], sum.f[i]) : sum.f[i] + y.f[i];
+        for (uint32_t j = CHOICES; j < p.k; j++) {
+          const uint32_t r = place_of(p, at + j);
+          if (r == kNowhere) continue;
+          y.from(ld_piece(row_at(p.row_in, p.row_in_stride, r), c));
+          if (WEIGHTED) sum.add(y, p.weights[at + j]);
+          else sum.add(y);
         }
-        st_piece<BYTES>(p.token_out, p.token_out_stride, t, c, sum.rounded());
+        st_piece(row_at(p.token_out, p.token_out_stride, t), c, sum.rounded());
       }
     }
-    const uint32_t width = min(group, 32u);
-#pragma unroll
-    for (int j = 0; j < kDots; j++)
-      for (uint32_t d = width >> 1; d; d >>= 1) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
-    if (group > 32) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-        for (int j = 0; j < kDots; j++) share[threadIdx.x >> 5][j] = dot[j];
-      }
-      __syncthreads();
-      if (in_group < kDots && live && j0 + in_group < p.k) {
-        float sum = 0.f;
-        for (uint32_t i = 0; i < group / 32; i++) sum += share[(threadIdx.x >> 5) + i][in_group];
-        p.dots[at + j0 + in_group] = sum;
-      }
-    } else if (live && in_group == 0) {
-#pragma unroll
-      for (int j = 0; j < kDots; j++)
-        if (j0 + j < p.k) p.dots[at + j0 + j] = dot[j];
-    }
+    share_sums<CHOICES>(dot, share, p, at, j0, live, lane, lanes);
   }
-  if (SPREAD) zero_tail<BYTES>(p, pieces);
+  if (SPREAD) zero_untaken(p, pieces);
 }
 
-// Widest piece of 16, 4 (or 2) bytes that divides the rows and every address and stride in use.
-int piece_bytes(const RouteRows& p, int elem_bytes) {
+// ---- rows off the 16-byte boundaries ---------------------------------------------------------
+// Rows of odd lengths start anywhere.  A row that is written is cut at its own 16-byte boundaries and stored in whole
+// pieces; what goes there is read from the other row as the two pieces that hold it, shifted into place.
+// (Elements one by one: 4097 x 3 rows of 1001 fp16 summed in 19.8 us.)
+
+// The 16 bytes at q (aligned), zeros outside [begin, end).
+__device__ __forceinline__ Piece piece_within(const char* q, const char* begin, const char* end) {
+  Piece p = {};
+  if (q >= begin && q + 16 <= end) {
+    p = *reinterpret_cast<const Piece*>(q);
+  } else if (q + 16 > begin && q < end) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const char* h = q + 2 * i;
+      const uint32_t x = h >= begin && h < end ? *reinterpret_cast<const uint16_t*>(h) : 0u;
+      p.v[i / 2] |= x << (i & 1 ? 16 : 0);
+    }
+  }
+  return p;
+}
+// The 16 bytes from `at` (an even address) on, zeros outside the row.
+__device__ __forceinline__ Piece piece_anywhere(const char* at, const char* begin, const char* end) {
+  const uintptr_t low = reinterpret_cast<uintptr_t>(at) & 15;
+  const char* q = at - low;
+  const Piece a = piece_within(q, begin, end);
+  if (low == 0) return a;
+  const Piece b = piece_within(q + 16, begin, end);
+  uint32_t w[8] = {a.v[0], a.v[1], a.v[2], a.v[3], b.v[0], b.v[1], b.v[2], b.v[3]};
+  if (low & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+  }
+  if (low & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+  }
+  Piece p;
+#pragma unroll
+  for (int i = 0; i < 4; i++) p.v[i] = low & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  return p;
+}
+template <typename E>
+__device__ __forceinline__ void store_within(char* q, const Piece& p, char* begin, char* end) {
+  if (q >= begin && q + 16 <= end) {
+    *reinterpret_cast<Piece*>(q) = p;
+    return;
+  }
+  const E* e = reinterpret_cast<const E*>(&p);
+#pragma unroll
+  for (int i = 0; i < Floats<E>::N; i++) {
+    char* h = q + i * sizeof(E);
+    if (h >= begin && h < end) *reinterpret_cast<E*>(h) = e[i];
+  }
+}
+
+// Piece `c` of a row that is written: its address, and how far it lies from the row's begin.
+struct Cut {
+  char *begin, *end, *at;
+  long long off;
+  __device__ __forceinline__ Cut(char* row, uint32_t bytes, uint32_t c) : begin(row), end(row + bytes) {
+    at = row - (reinterpret_cast<uintptr_t>(row) & 15) + (size_t)c * 16;
+    off = at - row;
+  }
+  __device__ __forceinline__ bool inside() const { return at < end; }
+};
+template <typename E>
+__device__ __forceinline__ Floats<E> read_at(const Cut& cut, const char* row, uint32_t bytes) {
+  Floats<E> x;
+  x.from(piece_anywhere(row + cut.off, row, row + bytes));
+  return x;
+}
+
+// lanes threads a token, as in dots_kernel; `pieces`: cuts of a row, at most.
+template <typename E, bool WEIGHTED, bool DOTS>
+__global__ void __launch_bounds__(kRowsBlock) gather_any_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
+  wait_for_launch_ahead();
+  release_launch_behind();
+  constexpr int kChoices = 4;
+  __shared__ float share[kRowsBlock / 32][kChoices];
+  const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E);
+  const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
+  const bool live = t < p.n_tokens;
+  const size_t at = (size_t)t * p.k;
+  for (uint32_t j0 = 0; j0 < (DOTS ? p.k : 1); j0 += kChoices) {
+    float dot[kChoices] = {};
+    for (uint32_t c = lane; live && c < pieces; c += lanes) {
+      const Cut cut(row_at(p.token_out, p.token_out_stride, t), bytes, c);
+      if (!cut.inside()) continue;
+      Floats<E> x, sum = {};
+      if (DOTS) x = read_at<E>(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+#pragma unroll
+      for (int j = 0; j < kChoices; j++) {
+        const uint32_t row = j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
+        if (row == kNowhere) continue;
+        const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
+        if (WEIGHTED) sum.add(y, p.weights[at + j0 + j]);
+        else sum.add(y);
+        if (DOTS) dot[j] = x.dot(y, dot[j]);
+      }
+      if (j0) continue;
+      for (uint32_t j = kChoices; j < p.k; j++) {  // choices past the first pass join the sum here, their products come later
+        const uint32_t row = place_of(p, at + j);
+        if (row == kNowhere) continue;
+        const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
+        if (WEIGHTED) sum.add(y, p.weights[at + j]);
+        else sum.add(y);
+      }
+      store_within<E>(cut.at, sum.rounded(), cut.begin, cut.end);
+    }
+    if (DOTS) share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
+  }
+}
+
+template <typename E, bool WEIGHTED, bool DOTS>
+__global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
+  wait_for_launch_ahead();
+  release_launch_behind();
+  constexpr int kChoices = 4;
+  __shared__ float share[kRowsBlock / 32][kChoices];
+  const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E);
+  const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
+  const bool live = t < p.n_tokens;
+  const size_t at = (size_t)t * p.k;
+  for (uint32_t j0 = 0; j0 < p.k; j0 += kChoices) {
+    float dot[kChoices] = {};
+    for (uint32_t c = lane; live && c < pieces; c += lanes) {
+#pragma unroll
+      for (int j = 0; j < kChoices; j++) {
+        const uint32_t row = j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
+        if (row == kNowhere) continue;
+        const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
+        if (!cut.inside()) continue;
+        const Floats<E> x = read_at<E>(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+        if (DOTS) dot[j] = x.dot(read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes), dot[j]);
+        store_within<E>(cut.at, WEIGHTED ? x.times(p.weights[at + j0 + j]).rounded() : x.rounded(), cut.begin, cut.end);
+      }
+    }
+    if (DOTS) share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
+  }
+  const uint32_t first = first_untaken(p);
+  const unsigned long long n = (unsigned long long)(p.n_rows - first) * pieces;
+  for (unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x; u < n;
+       u += (unsigned long long)gridDim.x * kRowsBlock) {
+    uint32_t row, c;
+    divide(u, pieces, &row, &c);
+    const Cut cut(row_at(p.row_out, p.row_out_stride, first + row), bytes, c);
+    if (cut.inside()) store_within<E>(cut.at, Piece{}, cut.begin, cut.end);
+  }
+}
+
+// Whether every row in use starts on a 16-byte boundary and is whole pieces long.
+bool rows_aligned(const RouteRows& p, int elem_bytes) {
   unsigned long long bits = (unsigned long long)p.dim * elem_bytes;
   auto add = [&](const void* q, long long stride) {
     if (q) bits |= reinterpret_cast<uintptr_t>(q) | (unsigned long long)stride;
@@ -448,43 +669,56 @@ int piece_bytes(const RouteRows& p, int elem_bytes) {
   add(p.token_out, p.token_out_stride);
   add(p.row_in, p.row_in_stride);
   add(p.row_out, p.row_out_stride);
-  return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+  return bits % 16 == 0;
 }
 
-template <typename E, int BYTES>
+// Threads that walk a row together: four pieces each, but a warp where the row has that many.
+uint32_t row_lanes(uint32_t pieces) {
+  uint32_t lanes = 1;
+  while (lanes < 32 ? lanes < pieces : lanes * 4 < pieces && lanes < (uint32_t)kRowsBlock) lanes *= 2;
+  return lanes;
+}
+
+template <typename E, bool WEIGHTED>
 cudaError_t rows_launch(const RouteRows& p, bool spread, cudaStream_t stream) {
-  const uint32_t pieces = (uint32_t)((unsigned long long)p.dim * sizeof(E) / BYTES);
-  const bool weighted = p.weights != nullptr;
+  const unsigned long long bytes = (unsigned long long)p.dim * sizeof(E);
+  auto per_token = [&](auto kern, uint32_t pieces) {
+    const uint32_t lanes = row_lanes(pieces), per = kRowsBlock / lanes;
+    return launch(kern, (p.n_tokens + per - 1) / per, kRowsBlock, 0, stream, true, p, pieces, lanes);
+  };
+  if (!rows_aligned(p, sizeof(E))) {
+    const uint32_t cuts = (uint32_t)((bytes + 15) / 16 + 1);
+    if (spread) return per_token(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, cuts);
+    return per_token(p.dots ? gather_any_kernel<E, WEIGHTED, true> : gather_any_kernel<E, WEIGHTED, false>, cuts);
+  }
+  const uint32_t pieces = (uint32_t)(bytes / 16);
   if (p.dots) {
-    uint32_t group = 1;
-    while (group < pieces && group < (uint32_t)kRowsBlock) group *= 2;
-    const uint32_t per = kRowsBlock / group, grid = (p.n_tokens + per - 1) / per;
-    auto kern = spread ? (weighted ? dots_kernel<E, BYTES, true, true> : dots_kernel<E, BYTES, false, true>)
-                       : (weighted ? dots_kernel<E, BYTES, true, false> : dots_kernel<E, BYTES, false, false>);
-    return launch(kern, grid, kRowsBlock, 0, stream, true, p, pieces, group);
+    if (spread)
+      return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, true, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, true, 4> : dots_kernel<E, WEIGHTED, true, 8>, pieces);
+    return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, false, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, false, 4> : dots_kernel<E, WEIGHTED, false, 8>, pieces);
   }
   const unsigned long long units = (unsigned long long)p.n_tokens * pieces;
-  const unsigned long long grid = (units + kRowsBlock - 1) / kRowsBlock;
-  if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-  auto kern = spread ? (weighted ? spread_kernel<E, BYTES, true> : spread_kernel<E, BYTES, false>)
-                     : (weighted ? gather_kernel<E, BYTES, true> : gather_kernel<E, BYTES, false>);
-  return launch(kern, (unsigned)grid, kRowsBlock, 0, stream, true, p, pieces);
+  auto per_piece = [&](auto kern, uint32_t each) {
+    const unsigned long long grid = (units / each + kRowsBlock - 1) / kRowsBlock;
+    return grid > 0x7fffffffull ? cudaErrorInvalidValue : launch(kern, (unsigned)grid, kRowsBlock, 0, stream, true, p, pieces);
+  };
+  if (spread) return per_piece(spread_kernel<E, WEIGHTED>, 1);
+  // eight loads in flight a thread, once there are threads enough to fill the GPU
+  const bool many = units >= 148ull * 2048 * 4;
+  if (p.k <= 2 && many && pieces % 4 == 0) return per_piece(gather_kernel<E, WEIGHTED, 2, 4>, 4);
+  if (p.k <= 4 && many && pieces % 2 == 0) return per_piece(gather_kernel<E, WEIGHTED, 4, 2>, 2);
+  return per_piece(gather_kernel<E, WEIGHTED, 8, 1>, 1);
 }
 
 cudaError_t rows_by_type(const RouteRows& p, int elem, bool spread, cudaStream_t stream) {
   if (p.n_tokens == 0) return cudaSuccess;
-  const int bytes = piece_bytes(p, elem == kElemF32 ? 4 : 2);
-  auto by_piece = [&](auto e) {
+  auto by_weight = [&](auto e) {
     using E = decltype(e);
-    if (bytes == 16) return rows_launch<E, 16>(p, spread, stream);
-    if constexpr (sizeof(E) == 2) {
-      if (bytes == 2) return rows_launch<E, 2>(p, spread, stream);
-    }
-    return rows_launch<E, 4>(p, spread, stream);
+    return p.weights ? rows_launch<E, true>(p, spread, stream) : rows_launch<E, false>(p, spread, stream);
   };
-  if (elem == kElemF32) return by_piece(float{});
-  if (elem == kElemF16) return by_piece(__half{});
-  return by_piece(__nv_bfloat16{});
+  if (elem == kElemF32) return by_weight(float{});
+  if (elem == kElemF16) return by_weight(__half{});
+  return by_weight(__nv_bfloat16{});
 }
 
 }  // namespace
