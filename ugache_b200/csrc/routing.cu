@@ -672,30 +672,30 @@ bool rows_aligned(const RouteRows& p, int elem_bytes) {
   return bits % 16 == 0;
 }
 
-// Threads that walk a row together: four pieces each, but a warp where the row has that many.
-uint32_t row_lanes(uint32_t pieces) {
+// Threads that walk a row together: `each` pieces a thread, but a warp where the row has that many.
+uint32_t row_lanes(uint32_t pieces, uint32_t each) {
   uint32_t lanes = 1;
-  while (lanes < 32 ? lanes < pieces : lanes * 4 < pieces && lanes < (uint32_t)kRowsBlock) lanes *= 2;
+  while (lanes < 32 ? lanes < pieces : lanes * each < pieces && lanes < (uint32_t)kRowsBlock) lanes *= 2;
   return lanes;
 }
 
 template <typename E, bool WEIGHTED>
 cudaError_t rows_launch(const RouteRows& p, bool spread, cudaStream_t stream) {
   const unsigned long long bytes = (unsigned long long)p.dim * sizeof(E);
-  auto per_token = [&](auto kern, uint32_t pieces) {
-    const uint32_t lanes = row_lanes(pieces), per = kRowsBlock / lanes;
+  auto per_token = [&](auto kern, uint32_t pieces, uint32_t each) {
+    const uint32_t lanes = row_lanes(pieces, each), per = kRowsBlock / lanes;
     return launch(kern, (p.n_tokens + per - 1) / per, kRowsBlock, 0, stream, true, p, pieces, lanes);
   };
   if (!rows_aligned(p, sizeof(E))) {
     const uint32_t cuts = (uint32_t)((bytes + 15) / 16 + 1);
-    if (spread) return per_token(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, cuts);
-    return per_token(p.dots ? gather_any_kernel<E, WEIGHTED, true> : gather_any_kernel<E, WEIGHTED, false>, cuts);
+    if (spread) return per_token(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, cuts, p.dots ? 2 : 1);
+    return per_token(p.dots ? gather_any_kernel<E, WEIGHTED, true> : gather_any_kernel<E, WEIGHTED, false>, cuts, p.dots ? 2 : 1);
   }
   const uint32_t pieces = (uint32_t)(bytes / 16);
   if (p.dots) {
     if (spread)
-      return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, true, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, true, 4> : dots_kernel<E, WEIGHTED, true, 8>, pieces);
-    return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, false, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, false, 4> : dots_kernel<E, WEIGHTED, false, 8>, pieces);
+      return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, true, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, true, 4> : dots_kernel<E, WEIGHTED, true, 8>, pieces, 4);
+    return per_token(p.k <= 2 ? dots_kernel<E, WEIGHTED, false, 2> : p.k <= 4 ? dots_kernel<E, WEIGHTED, false, 4> : dots_kernel<E, WEIGHTED, false, 8>, pieces, 4);
   }
   const unsigned long long units = (unsigned long long)p.n_tokens * pieces;
   auto per_piece = [&](auto kern, uint32_t each) {
@@ -706,8 +706,8 @@ cudaError_t rows_launch(const RouteRows& p, bool spread, cudaStream_t stream) {
   // eight loads in flight a thread, once there are threads enough to fill the GPU
   const bool many = units >= 148ull * 2048 * 4;
   if (p.k <= 2 && many && pieces % 4 == 0) return per_piece(gather_kernel<E, WEIGHTED, 2, 4>, 4);
-  if (p.k <= 4 && many && pieces % 2 == 0) return per_piece(gather_kernel<E, WEIGHTED, 4, 2>, 2);
-  return per_piece(gather_kernel<E, WEIGHTED, 8, 1>, 1);
+  if (many && pieces % 2 == 0) return per_piece(gather_kernel<E, WEIGHTED, 4, 2>, 2);
+  return per_piece(gather_kernel<E, WEIGHTED, 4, 1>, 1);
 }
 
 cudaError_t rows_by_type(const RouteRows& p, int elem, bool spread, cudaStream_t stream) {
