@@ -126,7 +126,7 @@ constexpr uint32_t kPlanCluster = 8;
 // part p in its cluster; rows of n_groups + 1.
 template <typename IdT>
 __global__ void __launch_bounds__(kPlanBlock) plan_count_kernel(const IdT* __restrict__ ids, uint32_t n, uint32_t n_groups,
-                                                                uint32_t part, uint32_t bits, uint32_t* __restrict__ totals,
+                                                                uint32_t part, uint32_t* __restrict__ totals,
                                                                 uint32_t* __restrict__ ahead) {
   extern __shared__ uint32_t hist[];
   wait_for_launch_ahead();
@@ -143,10 +143,8 @@ __global__ void __launch_bounds__(kPlanBlock) plan_count_kernel(const IdT* __res
       group[k] = i < end ? group_of(ids[i], n_groups) : kNoId;
     }
 #pragma unroll
-    for (int k = 0; k < kPlanSteps; k++) {
-      const unsigned same = lanes_of_group(group[k], group[k] != kNoId, bits);
-      if (group[k] != kNoId && (threadIdx.x & 31) == (uint32_t)__ffs(same) - 1) atomicAdd(&hist[group[k]], __popc(same));
-    }
+    for (int k = 0; k < kPlanSteps; k++)  // at worst, all in one group, a lane at a time: as long as the ballots would take
+      if (group[k] != kNoId) atomicAdd(&hist[group[k]], 1u);
   }
   cluster_arrive();
   cluster_wait();
@@ -177,11 +175,12 @@ __global__ void __launch_bounds__(kPlanBlock)
                       const uint32_t* ahead_in_cluster,
                       int32_t* __restrict__ offsets, int32_t* __restrict__ order, int32_t* __restrict__ position) {
   extern __shared__ uint32_t smem[];
-  __shared__ uint32_t partial[32], ahead[SHARED == Shared::kNot ? 1 : kRouteMaxGroups + 1];
+  __shared__ uint32_t partial[32], ahead[SHARED == Shared::kNot ? 1 : kRouteMaxGroups + 1], local[SHARED == Shared::kNot ? 1 : kRouteMaxGroups + 1];
   const uint32_t G1 = n_groups + 1, n_warp = blockDim.x >> 5;
   uint32_t* start = smem;                                       // [G1] the tile's first place of each group
   uint32_t* count = smem + G1;                                  // [G1] ids of the tile
-  uint16_t* seen = reinterpret_cast<uint16_t*>(smem + 2 * G1 + (G1 & 1) * 2);  // [n_warp][G1], 8-byte aligned
+  uint16_t* seen = reinterpret_cast<uint16_t*>(smem + 2 * G1);  // [n_warp][G1], 8-byte aligned
+  uint2* sorted = reinterpret_cast<uint2*>(smem + 2 * G1);      // later: the tile's ids in order, each with its place
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint16_t* mine = seen + (size_t)warp * G1;
   const uint32_t begin = min(n, blockIdx.x * part), end = min(n, begin + part);
@@ -267,13 +266,33 @@ __global__ void __launch_bounds__(kPlanBlock)
       first = false;
     }
     __syncthreads();
+    if (SHARED != Shared::kNot) {
+      for (uint32_t g = threadIdx.x; g < G1; g += blockDim.x) local[g] = count[g];
+      __syncthreads();
+      block_exclusive_scan(local, G1, partial);
+    }
+    // in order through shared memory, so that a group's ids leave together
+    uint32_t place[kPlanSteps];
 #pragma unroll
     for (int s = 0; s < kPlanSteps; s++) {
       const uint32_t g = group[s];
       if ((uint32_t)s >= steps || g == kNoId) break;  // a run's ids are a prefix of its lanes' steps
-      const uint32_t i = run + s * 32 + lane, at = start[g] + mine[g] + rank[s];
-      order[at] = (int32_t)i;
-      position[i] = g < n_groups ? (int32_t)at : -1;
+      rank[s] += mine[g];
+      place[s] = start[g] + rank[s];
+      if (SHARED != Shared::kNot) rank[s] += local[g];
+      else rank[s] = place[s];
+      position[run + s * 32 + lane] = g < n_groups ? (int32_t)place[s] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kPlanSteps; s++) {
+      if ((uint32_t)s >= steps || group[s] == kNoId) break;
+      sorted[rank[s]] = make_uint2(run + s * 32 + lane, place[s]);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(end - min(tile, end), blockDim.x * steps); i += blockDim.x) {
+      const uint2 id = sorted[i];
+      order[id.y] = (int32_t)id.x;
     }
     __syncthreads();
     if (SHARED == Shared::kParts)
@@ -830,7 +849,8 @@ cudaError_t launch_route_plan(const void* ids, int id_bytes, uint32_t n, int n_g
   const uint32_t G = (uint32_t)n_groups;
   uint32_t bits = 0;
   while (G >> bits) bits++;  // groups 0 .. G: G is that of the ids without one
-  const size_t smem = (size_t)(G + 1) * (2 * sizeof(uint32_t) + (s.block / 32) * sizeof(uint16_t)) + 16;
+  const size_t tile = std::min(s.part, s.block * kPlanSteps);
+  const size_t smem = (size_t)(G + 1) * 2 * sizeof(uint32_t) + std::max((G + 1) * (s.block / 32) * sizeof(uint16_t) + 8, tile * sizeof(uint2));
   auto go = [&](auto id) {
     using IdT = decltype(id);
     const IdT* in = static_cast<const IdT*>(ids);
@@ -842,7 +862,7 @@ cudaError_t launch_route_plan(const void* ids, int id_bytes, uint32_t n, int n_g
     if (s.shared == Shared::kNot) return place(plan_place_kernel<IdT, Shared::kNot>, 1);
     if (s.shared == Shared::kCluster) return place(plan_place_kernel<IdT, Shared::kCluster>, kPlanCluster);
     cudaError_t e = launch(plan_count_kernel<IdT>, s.parts, kPlanBlock, (G + 1) * sizeof(uint32_t), stream, true, kPlanCluster, in, n, G,
-                           s.part, bits, totals, ahead);
+                           s.part, totals, ahead);
     return e == cudaSuccess ? place(plan_place_kernel<IdT, Shared::kParts>, 1) : e;
   };
   return id_bytes == 8 ? go((long long)0) : go((int32_t)0);
