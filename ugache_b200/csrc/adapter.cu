@@ -511,7 +511,15 @@ __device__ __forceinline__ void from_tensor_memory(float (&v)[16], uint32_t at) 
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(at));
 }
-__device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The loads into v have landed (v passes through, so that nothing reads it ahead of this).
+template <int N>
+__device__ __forceinline__ void loads_done(float (&v)[N][16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < N; c++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) asm volatile("" : "+f"(v[c][i]));
+}
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -712,14 +720,18 @@ __global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterPa
       const uint32_t part = blockIdx.x - (uint32_t)((unsigned long long)(run.first + n) * run.tile_steps / share.run(run.tiles));
       float* to = inner + ((size_t)part * p.n_tokens + tile.first) * RP + row * 4;
 #pragma unroll
-      for (int c = 0; c < RP; c += 16) {
-        float v[16];
-        from_tensor_memory(v, tmem + ((warp - 4) * 32 << 16) + (n & 1) * RP + c);
-        loads_done();
+      for (int c0 = 0; c0 < RP; c0 += 64) {
+        constexpr int kLoads = RP < 64 ? RP / 16 : 4;
+        float v[kLoads][16];
+#pragma unroll
+        for (int c = 0; c < kLoads; c++) from_tensor_memory(v[c], tmem + ((warp - 4) * 32 << 16) + (n & 1) * RP + c0 + c * 16);
+        loads_done(v);
         if (row < tile.count) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(to + (size_t)(c + i) * tile.count) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int c = 0; c < kLoads; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(to + (size_t)(c0 + c * 16 + i) * tile.count) = make_float4(v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3]);
         }
       }
       before_sync();
@@ -759,6 +771,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, BigShare down_share, BigShare share) {
   using S = BigShape<RP>;
   constexpr int kStages = S::kUpStages, kColumns = 2 * kStep;
+  // pieces a thread takes out at once: with two stages the ring waits for them (rank 128: 16,384 prompts 119 us against
+  // 133 with four), with more the registers count
+  constexpr int kWide = kStages == 2 ? 8 : 4;
   extern __shared__ unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kStages], drained[kStages], product[2], taken[2], terms, tops;
   __shared__ uint32_t tmem_slot;
@@ -890,26 +905,29 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         if (!ok) break;
         after_sync();
 #pragma unroll
-        for (int c = 0; c < 8; c += 2) {
-          float v[16];
-          from_tensor_memory(v, tmem + (quarter * 32 << 16) + (i & 1) * kStep + half * 64 + c * 8);
-          uint32_t w[2][4];
+        for (int c0 = 0; c0 < 8; c0 += kWide) {
+          float v[kWide / 2][16];
 #pragma unroll
-          for (int h = 0; h < 2; h++)
+          for (int c = 0; c < kWide / 2; c++)
+            from_tensor_memory(v[c], tmem + (quarter * 32 << 16) + (i & 1) * kStep + half * 64 + c0 * 8 + c * 16);
+          uint32_t w[kWide][4];
+#pragma unroll
+          for (int c = 0; c < kWide; c++)
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[h][0]), "=r"(w[h][1]), "=r"(w[h][2]), "=r"(w[h][3])
-                         : "r"(at + block + piece_at(row, c + h))
+                         : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3])
+                         : "r"(at + block + piece_at(row, c0 + c))
                          : "memory");
-          loads_done();
+          loads_done(v);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
+          for (int c = 0; c < kWide; c++) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              const float2 b = Half<E>::widen(w[h][j]);
-              w[h][j] = Half<E>::narrow(fmaf(v[8 * h + 2 * j], back, b.x), fmaf(v[8 * h + 2 * j + 1], back, b.y));
+              const float2 b = Half<E>::widen(w[c][j]);
+              const float* d = &v[c / 2][c % 2 * 8 + 2 * j];
+              w[c][j] = Half<E>::narrow(fmaf(d[0], back, b.x), fmaf(d[1], back, b.y));
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + block + piece_at(row, c + h)), "r"(w[h][0]),
-                         "r"(w[h][1]), "r"(w[h][2]), "r"(w[h][3])
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + block + piece_at(row, c0 + c)), "r"(w[c][0]),
+                         "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3])
                          : "memory");
           }
         }
