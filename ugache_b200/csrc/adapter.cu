@@ -163,8 +163,8 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
 
 constexpr int kMostCluster = 8;
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Columns [begin, end) of the tokens' rows from one matrix to another; by the whole CTA, four pieces a thread in flight.
 template <int ROWS, bool VECTOR>
@@ -368,6 +368,7 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   __syncthreads();
   cluster_arrive();  // waited for at the end: nobody leaves while its sums are being read
   if (held) barrier_wait(shared_address(&up_landed), 0);
+  __syncwarp();
 
   // second product: every CTA a slice of out_dim, 32 of it a warp at a time.  Column 2c + b of the
   // q-th of four matrix tiles is output 8c + 2q + b, so that a lane ends with 8 consecutive outputs.
@@ -460,6 +461,8 @@ constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, m
 constexpr int kUpThreads = kProducers + 256 + 32;
 constexpr int kMostTiles = 36;                              // a CTA's run touches
 
+// By a whole warp, which stays together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(kFull, barrier_wait(bar, parity)); }
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterPa
     const uint32_t row = threadIdx.x - kProducers;
     for (uint32_t n = 0; n < run.count; n++) {
       const Tile tile = tiles[n];
-      if (!barrier_wait(shared_address(&ready[n & 1]), n / 2 & 1)) break;
+      if (!warp_wait(shared_address(&ready[n & 1]), n / 2 & 1)) break;
       after_sync();
       const uint32_t part = blockIdx.x - (uint32_t)((unsigned long long)(run.first + n) * run.tile_steps / share.run(run.tiles));
       float* to = inner + ((size_t)part * p.n_tokens + tile.first) * RP + row * 4;
@@ -763,6 +766,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterPa
   before_sync();
   __syncthreads();
   after_sync();
+  __syncwarp();
   if (warp == 8) free_tensor_memory<kColumns>(tmem);
 }
 
@@ -871,7 +875,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         }
         top_of[half][row] = top;
         barrier_arrive(shared_address(&tops));
-        if (!(ok = barrier_wait(shared_address(&tops), n & 1))) break;
+        if (!(ok = warp_wait(shared_address(&tops), n & 1))) break;
         const float s = unit_scale(fmaxf(top, top_of[half ^ 1][row]));
         back = 1.f / s;
 #pragma unroll
@@ -901,7 +905,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       }
       for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
         const uint32_t s = i % kStages, at = ring + s * S::kUpStage, column = k * kStep;
-        ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) && barrier_wait(shared_address(&product[i & 1]), i / 2 & 1);
+        ok = warp_wait(shared_address(&full[s]), i / kStages & 1) && warp_wait(shared_address(&product[i & 1]), i / 2 & 1);
         if (!ok) break;
         after_sync();
 #pragma unroll
@@ -975,6 +979,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   before_sync();
   __syncthreads();
   after_sync();
+  __syncwarp();
   if (warp == 12) free_tensor_memory<kColumns>(tmem);
 }
 

@@ -17,8 +17,8 @@ constexpr unsigned kFull = 0xffffffffu;
 __device__ __forceinline__ void wait_for_launch_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_launch_behind() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // A word of shared memory as CTA `rank` of the cluster has it at the same place.
 __device__ __forceinline__ uint32_t count_of(const uint32_t* mine, uint32_t rank) {
   uint32_t at, v;
@@ -685,10 +685,13 @@ struct Cut {
   }
   __device__ __forceinline__ bool inside() const { return at < end; }
 };
+__device__ __forceinline__ Piece piece_of(const Cut& cut, const char* row, uint32_t bytes) {
+  return piece_anywhere(row + cut.off, row, row + bytes, cut.off >= 16 && cut.at + 32 <= cut.end);
+}
 template <typename E>
 __device__ __forceinline__ Floats<E> read_at(const Cut& cut, const char* row, uint32_t bytes) {
   Floats<E> x;
-  x.from(piece_anywhere(row + cut.off, row, row + bytes, cut.off >= 16 && cut.at + 32 <= cut.end));
+  x.from(piece_of(cut, row, bytes));
   return x;
 }
 
@@ -754,9 +757,11 @@ __global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uin
         if (row == kNowhere) continue;
         const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
         if (!cut.inside()) continue;
-        const Floats<E> x = read_at<E>(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+        const Piece in = piece_of(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+        Floats<E> x;
+        x.from(in);
         if (DOTS) dot[j] = x.dot(read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes), dot[j]);
-        store_within<E>(cut.at, WEIGHTED ? x.times(p.weights[at + j0 + j]).rounded() : x.rounded(), cut.begin, cut.end);
+        store_within<E>(cut.at, WEIGHTED ? x.times(p.weights[at + j0 + j]).rounded() : in, cut.begin, cut.end);
       }
     }
     if (DOTS) share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
