@@ -245,6 +245,40 @@ def test_captured_and_replayed(rt, T):
         assert bool(((out.double() - want).abs() <= slack).all())
 
 
+@pytest.mark.parametrize("T", [64, 2700])
+def test_bad_plans_stay_in_bounds(rt, T):
+    """Tokens outside the batch are skipped and offsets clamped, whatever a caller put there."""
+    c = Case(rt, T, 4, 16, 256, 128, "bf16", none=0.0)
+    want, slack = formula(c.base, c.x, c.down, c.up, c.ids, c.scale)
+    order = c.plan.order.clone()
+    gone = order[[1, T // 2, T - 1]].long()
+    order[1], order[T // 2], order[T - 1] = -1, T, 1 << 30
+    out = torch.full_like(c.base, 9.0)
+    rt.adapter_add(c.base, c.x, c.down, c.up, c.plan._replace(order=order), scale=c.scale, out=out)
+    kept = torch.ones(T, dtype=torch.bool, device="cuda")
+    kept[gone] = False
+    assert bool(((out.double() - want).abs() <= slack)[kept].all()) and bool((out[gone] == 9.0).all())
+    offsets = c.plan.offsets.clone()
+    offsets[-1] = 1 << 30        # beyond the batch: as if it were its end
+    assert torch.equal(rt.adapter_add(c.base, c.x, c.down, c.up, c.plan._replace(offsets=offsets), scale=c.scale),
+                       rt.adapter_add(c.base, c.x, c.down, c.up, c.plan, scale=c.scale))
+
+
+def test_two_streams_at_once(rt):
+    """Prompts and single tokens side by side: the calls share nothing."""
+    big, small = Case(rt, 6000, 6, 64, 1024, 1024, "bf16"), Case(rt, 64, 9, 16, 1024, 1024, "bf16")
+    run = lambda c: rt.adapter_add(c.base, c.x, c.down, c.up, c.plan, scale=c.scale)  # noqa: E731
+    want = [run(big), run(small)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 4]):
+            got.append((i % 2, run((big, small)[i % 2])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for k, y in got)
+
+
 def test_adapters_behind_the_cache(rt):
     """The run as a server makes it: adapters are rows of a table in host memory, the hot ones cached; a batch's
     distinct adapters are looked up once and applied through the lookup's own index."""

@@ -406,6 +406,86 @@ def test_captured_and_replayed(rt):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_behind_lookups_in_one_stream(rt):
+    """Tokens' rows from the cache, routed, and looked up again from what the routing wrote: every kernel waits for the ones
+    ahead of it, however they overlap."""
+    N, dim, n = 4000, 64, 512
+    table = torch.randn(N, dim).pin_memory()
+    cache = rt.Cache(1, N, dim * 4, 0.9, max_batch=4096)
+    cache.set_placement(rt.solve_placement("rep", 1, np.arange(N, dtype=np.uint32), None, 90.0))
+    cache.build(0, 0, table.data_ptr())
+    dev = table.cuda()
+    keys = torch.randint(0, N, (n,), device="cuda")
+    ids = torch.randint(0, 7, (n, 2), device="cuda")
+    for _ in range(30):
+        x = cache.lookup(0, keys).view(torch.float32)
+        plan = rt.route_plan(ids, 7)
+        y = rt.route_combine(rt.route_dispatch(x, plan), plan)
+        again = cache.lookup(0, plan.order[:n] % N).view(torch.float32)     # keys that the plan has just written
+        pooled = cache.lookup_pool(0, plan.order, bag_size=2)
+        assert torch.equal(y, 2 * dev[keys])
+        assert torch.equal(again, dev[plan.order[:n].long()])
+        assert torch.equal(pooled, dev[plan.order.long()].view(n, 2, dim).sum(1))
+        keys = plan.order[n:].long() % N
+    out = torch.empty(n, dim, device="cuda")
+    with pytest.raises(rt.UgcError):   # bf16 rows are routed, not pooled
+        cache.lookup_pool_ptr(0, keys.data_ptr(), 8, n, 0, n, 1, 2, 0, out.data_ptr())
+    cache.close()
+
+
+def test_a_layer_under_autograd(rt):
+    """Dispatch, experts and combine as a training step uses them, against the same layer in 64 bits.  Every value is
+    sums of products of at most 7 factors: off by at most (terms + 8) * 2^-24 of what the layer gives for the magnitudes."""
+    class Dispatch(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, plan):
+            ctx.plan = plan
+            return rt.route_dispatch(x, plan)
+
+        @staticmethod
+        def backward(ctx, g):
+            return rt.route_dispatch_grad(g, ctx.plan)[0], None
+
+    class Combine(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, rows, weights, plan):
+            ctx.plan = plan
+            ctx.save_for_backward(rows, weights)
+            return rt.route_combine(rows, plan, weights=weights)
+
+        @staticmethod
+        def backward(ctx, g):
+            rows, weights = ctx.saved_tensors
+            return (*rt.route_combine_grad(g, ctx.plan, weights=weights, rows=rows), None)
+
+    T, k, G, dim = 200, 3, 6, 72
+    g = torch.Generator(device="cuda")
+    g.manual_seed(11)
+    ids = torch.randint(-1, G, (T, k), generator=g, device="cuda")
+    plan = rt.route_plan(ids, G)
+    routed = int(plan.offsets[-1])
+    group = ids.reshape(-1)[plan.order[:routed].long()]
+    x, w, expert, up = (torch.randn(*s, generator=g, device="cuda") for s in ((T, dim), (T, k), (G, dim), (T, dim)))
+
+    def fused(x, w, expert):
+        rows = Dispatch.apply(x, plan)
+        out = torch.cat([rows[:routed] * expert[group], rows[routed:]])
+        return Combine.apply(out, w, plan)
+
+    def plain(x, w, expert):
+        return sum(torch.where((ids[:, j] >= 0)[:, None], w[:, j, None] * (x * expert[ids[:, j].clamp(min=0)]), 0.0) for j in range(k))
+
+    def gradients(layer, ty, change=lambda t: t):
+        leaves = [change(t.to(ty)).detach().requires_grad_() for t in (x, w, expert)]
+        y = layer(*leaves)
+        y.backward(change(up.to(ty)))
+        return [y.detach()] + [t.grad for t in leaves]
+
+    got, want, size = gradients(fused, torch.float32), gradients(plain, torch.float64), gradients(plain, torch.float64, torch.abs)
+    for a, b, m, terms in zip(got, want, size, (k, k, dim, T * k)):
+        assert bool(((a.double() - b).abs() <= (terms + 8) * U * m).all())
+
+
 def test_same_results_again(rt):
     c = Case(rt, 2000, 8, 1000, "f16")
     first = rt.route_dispatch_grad(c.rows, c.plan, weights=c.w, x=c.x)

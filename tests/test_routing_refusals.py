@@ -97,7 +97,3 @@ def test_adapter_workspace(L):
 def test_adapter_no_tokens(L):
     assert adapter(L, tokens=0, base=None, x=None, down=None, up=None, offsets=None, order=None, out=None) == 0
 
-
-def test_pooled_lookup_keeps_refusing_bf16(L):
-    # no context: the call is refused before the element type is looked at; the type itself is checked on the GPU
-    assert L.ugc_lookup_pool(None, 0, A, 8, 4, None, 2, 2, 2, 0, B, None) != 0
