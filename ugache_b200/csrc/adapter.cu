@@ -166,27 +166,31 @@ constexpr int kMostCluster = 8;
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// Columns [begin, end) of the tokens' rows from one matrix to another; by the whole CTA, four pieces a thread in flight.
-template <int ROWS, bool VECTOR>
-__device__ __forceinline__ void copy_rows(const uint16_t* from, long long from_stride, uint16_t* to, long long to_stride,
-                                          const int32_t* token, uint32_t count, uint32_t begin, uint32_t end) {
+// Columns [begin, end) of the rows of a tile's tokens from one matrix to another; by THREADS threads, four pieces each in
+// flight.  token(m): the m-th token of the tile, negative for none.
+template <int THREADS, bool VECTOR, typename Token>
+__device__ __forceinline__ void copy_rows(const AdapterParams& p, Token token, uint32_t count, uint32_t begin, uint32_t end,
+                                          uint32_t thread) {
   constexpr uint32_t kPiece = VECTOR ? 8 : 1;
+  const uint16_t* from = static_cast<const uint16_t*>(p.base);
+  uint16_t* to = static_cast<uint16_t*>(p.out);
   const uint32_t pieces = (end - begin + kPiece - 1) / kPiece, all = count * pieces;
-  for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 4 * kBlock) {
+  for (uint32_t i0 = thread; i0 < all; i0 += 4 * THREADS) {
     uint4 v[4];
+    int t[4];
+#pragma unroll
+    for (int f = 0; f < 4; f++) t[f] = i0 + f * THREADS < all ? token((i0 + f * THREADS) / pieces) : -1;
 #pragma unroll
     for (int f = 0; f < 4; f++) {
-      const uint32_t i = i0 + f * kBlock, m = i / pieces, n = begin + i % pieces * kPiece;
-      if (i >= all || token[m] < 0) continue;
-      const uint16_t* at = from + (long long)token[m] * from_stride + n;
+      if (t[f] < 0) continue;
+      const uint16_t* at = from + (long long)t[f] * p.base_stride + begin + (i0 + f * THREADS) % pieces * kPiece;
       if (VECTOR) v[f] = *reinterpret_cast<const uint4*>(at);
       else v[f].x = *at;
     }
 #pragma unroll
     for (int f = 0; f < 4; f++) {
-      const uint32_t i = i0 + f * kBlock, m = i / pieces, n = begin + i % pieces * kPiece;
-      if (i >= all || token[m] < 0) continue;
-      uint16_t* at = to + (long long)token[m] * to_stride + n;
+      if (t[f] < 0) continue;
+      uint16_t* at = to + (long long)t[f] * p.out_stride + begin + (i0 + f * THREADS) % pieces * kPiece;
       if (VECTOR) *reinterpret_cast<uint4*>(at) = v[f];
       else *at = (uint16_t)v[f].x;
     }
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 
   if (bare) {  // no adapter
     if (out == base) return;
-    copy_rows<kTile, VECTOR>(base, p.base_stride, out, p.out_stride, token, tile.count, n_begin, n_end);
+    copy_rows<kBlock, VECTOR>(p, [&](uint32_t m) { return token[m]; }, tile.count, n_begin, n_end, threadIdx.x);
     return;
   }
   // first product: every CTA a slice of dim, 32 of it a warp at a time, several such loads in flight
@@ -815,7 +819,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     bool ok = true;
     for (uint32_t n = 0; ok && n < run.count; n++) {
       const Tile tile = tiles[n];
-      if (tile.group == p.n_groups) break;  // these come last
+      const bool bare = tile.group == p.n_groups;  // no adapter: these tiles come last, their rows just pass through
       RowCopies base;
       base.set(p.base, p.base_stride, p, tile);
       const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         if (i >= kStages && !(ok = barrier_wait(shared_address(&drained[s]), (i / kStages - 1) & 1))) break;
         const uint32_t to = ring + s * S::kUpStage, column = k * kStep;
         base.issue(to, column, p.out_dim);
-        copy_matrix<kStep, RP / 8>(to + kRowsBytes, up, p.rank, column, p.out_dim, 0, p.rank);
+        if (!bare) copy_matrix<kStep, RP / 8>(to + kRowsBytes, up, p.rank, column, p.out_dim, 0, p.rank);
         arrive_behind_copies(shared_address(&full[s]));
       }
     }
@@ -838,20 +842,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     bool ok = true;
     for (uint32_t n = 0; ok && n < run.count; n++) {
       const Tile tile = tiles[n];
-      if (tile.group == p.n_groups) {  // no adapter
-        const uint16_t* base = static_cast<const uint16_t*>(p.base);
-        const uint32_t begin = run.from(n) * kStep, end = min(p.out_dim, run.to(n) * kStep);
-        for (uint32_t m = warp - 4; m < tile.count; m += 8) {
-          const int t = token_at(p, tile, m);
-          if (t < 0) continue;
-          for (uint32_t c = begin + lane * 8; c < end; c += 256)
-            *reinterpret_cast<uint4*>(out + (long long)t * p.out_stride + c) =
-                *reinterpret_cast<const uint4*>(base + (long long)t * p.base_stride + c);
-        }
-        continue;
-      }
-      float back;
-      {  // half of the token's rank products a thread: added up, scaled so that the token's largest is in [1, 2), in two terms
+      const bool bare = tile.group == p.n_groups;
+      float back = 1.f;
+      if (!bare) {  // half of the token's rank products a thread: added up, scaled so that the token's largest is in [1, 2), in two terms
         constexpr int R = RP / 2;
         const float scale = p.scale ? p.scale[tile.group] : 1.f;
         const uint32_t per = down_share.run(run.tiles);
@@ -895,8 +888,10 @@ __global__ void __launch_bounds__(kUpThreads, 1)
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to2), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
         }
       }
-      order_for_tensor_cores();
-      barrier_arrive(shared_address(&terms));
+      if (!bare) {
+        order_for_tensor_cores();
+        barrier_arrive(shared_address(&terms));
+      }
       uint16_t* to[8];  // on the way out the thread has one piece of eight rows
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -905,11 +900,11 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       }
       for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
         const uint32_t s = i % kStages, at = ring + s * S::kUpStage, column = k * kStep;
-        ok = warp_wait(shared_address(&full[s]), i / kStages & 1) && warp_wait(shared_address(&product[i & 1]), i / 2 & 1);
+        ok = warp_wait(shared_address(&full[s]), i / kStages & 1) && (bare || warp_wait(shared_address(&product[i & 1]), i / 2 & 1));
         if (!ok) break;
         after_sync();
 #pragma unroll
-        for (int c0 = 0; c0 < 8; c0 += kWide) {
+        for (int c0 = 0; c0 < 8 && !bare; c0 += kWide) {
           float v[kWide / 2][16];
 #pragma unroll
           for (int c = 0; c < kWide / 2; c++)
@@ -937,7 +932,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         }
         before_sync();
         __syncwarp();
-        if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
+        if (lane == 0 && !bare) barrier_arrive(shared_address(&taken[i & 1]));
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           uint32_t w[4];

@@ -737,35 +737,28 @@ __global__ void __launch_bounds__(kRowsBlock) gather_any_kernel(RouteRows p, uin
   }
 }
 
+// lanes threads a choice: the rows written are cut differently.
 template <typename E, bool WEIGHTED, bool DOTS>
 __global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
   wait_for_launch_ahead();
   release_launch_behind();
-  constexpr int kChoices = 4;
-  __shared__ float share[kRowsBlock / 32][kChoices];
+  __shared__ float share[kRowsBlock / 32][1];
   const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E);
-  const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
-  const bool live = t < p.n_tokens;
-  const size_t at = (size_t)t * p.k;
-  for (uint32_t j0 = 0; j0 < p.k; j0 += kChoices) {
-    float dot[kChoices] = {};
-    for (uint32_t u = lane; live && u < pieces; u += lanes) {
-      const uint32_t c = u + 1 < pieces ? u + 1 : 0;
-#pragma unroll
-      for (int j = 0; j < kChoices; j++) {
-        const uint32_t row = j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
-        if (row == kNowhere) continue;
-        const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
-        if (!cut.inside()) continue;
-        const Piece in = piece_of(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
-        Floats<E> x;
-        x.from(in);
-        if (DOTS) dot[j] = x.dot(read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes), dot[j]);
-        store_within<E>(cut.at, WEIGHTED ? x.times(p.weights[at + j0 + j]).rounded() : in, cut.begin, cut.end);
-      }
-    }
-    if (DOTS) share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
+  const uint32_t choice = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes, t = choice / p.k;
+  const uint32_t row = choice < p.n_rows ? place_of(p, choice) : kNowhere;
+  const float w = WEIGHTED && row != kNowhere ? p.weights[choice] : 1.f;
+  float dot[1] = {};
+  for (uint32_t u = lane; row != kNowhere && u < pieces; u += lanes) {
+    const uint32_t c = u + 1 < pieces ? u + 1 : 0;
+    const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
+    if (!cut.inside()) continue;
+    const Piece in = piece_of(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+    Floats<E> x;
+    x.from(in);
+    if (DOTS) dot[0] = x.dot(read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes), dot[0]);
+    store_within<E>(cut.at, WEIGHTED ? x.times(w).rounded() : in, cut.begin, cut.end);
   }
+  if (DOTS) share_sums<1>(dot, share, p, choice, 0, choice < p.n_rows, lane, lanes);
   const uint32_t first = first_untaken(p);
   const unsigned long long n = (unsigned long long)(p.n_rows - first) * pieces;
   for (unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x; u < n;
@@ -802,13 +795,14 @@ uint32_t row_lanes(uint32_t pieces, uint32_t each) {
 template <typename E, bool WEIGHTED>
 cudaError_t rows_launch(const RouteRows& p, bool spread, cudaStream_t stream) {
   const unsigned long long bytes = (unsigned long long)p.dim * sizeof(E);
-  auto per_token = [&](auto kern, uint32_t pieces, uint32_t each) {
+  auto per_row = [&](auto kern, uint32_t rows, uint32_t pieces, uint32_t each) {
     const uint32_t lanes = row_lanes(pieces, each), per = kRowsBlock / lanes;
-    return launch(kern, (p.n_tokens + per - 1) / per, kRowsBlock, 0, stream, true, 1, p, pieces, lanes);
+    return launch(kern, (rows + per - 1) / per, kRowsBlock, 0, stream, true, 1, p, pieces, lanes);
   };
+  auto per_token = [&](auto kern, uint32_t pieces, uint32_t each) { return per_row(kern, p.n_tokens, pieces, each); };
   if (!rows_aligned(p, sizeof(E))) {
     const uint32_t cuts = (uint32_t)((bytes + 15) / 16 + 1);
-    if (spread) return per_token(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, cuts, p.dots ? 2 : 1);
+    if (spread) return per_row(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, p.n_rows, cuts, p.dots ? 2 : 4);
     return per_token(p.dots ? gather_any_kernel<E, WEIGHTED, true> : gather_any_kernel<E, WEIGHTED, false>, cuts, p.dots ? 2 : 1);
   }
   const uint32_t pieces = (uint32_t)(bytes / 16);
