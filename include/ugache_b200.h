@@ -452,7 +452,8 @@ int ugc_route_plan(int device_id, const void* ids, int id_bytes, size_t n_tokens
  *                  dweights[t,j] = <dy[t], rows[position[t,j]]>      (only if dweights is given)
  *
  * Sums and products are fp32, the choices of a token added in their order by fused multiply-adds,
- * one rounding at the end; results do not depend on the launch.  A choice whose position is -1 (or
+ * one rounding at the end; the order of the additions of dweights is fixed by dim, k and whether all rows
+ * start on 16-byte boundaries, never by the number of tokens.  A choice whose position is -1 (or
  * outside the rows) adds nothing, its row is not read and its dweights are 0; a token without any
  * choice gets zeros.  Rows of `out` and `drows` from `routed` on, which no choice takes, are zeroed;
  * routed NULL: left as they were.  x / rows may be NULL in the gradients if dweights is. */
@@ -479,7 +480,8 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
  * out may be base itself (same stride); other overlaps are not allowed.  fp16 and bf16, rank at most
  * UGC_ADAPTER_MAX_RANK; 16-byte aligned addresses and strides, dims and ranks in multiples of 8
  * elements take the fast loads.  Sums are fp32; the rank products enter the second product as two
- * 16-bit terms (16 significand bits or more).  workspace: ugc_adapter_workspace bytes (0 for small
+ * 16-bit terms (16 significand bits or more); infinities in an adapter that a token uses may come out as
+ * NaN.  workspace: ugc_adapter_workspace bytes (0 for small
  * batches, then NULL will do), 16-byte aligned, free again when the call's work is done. */
 #define UGC_ADAPTER_MAX_RANK 128
 int ugc_adapter_workspace(size_t n_tokens, int n_groups, size_t rank, size_t dim, size_t out_dim, size_t* bytes);
