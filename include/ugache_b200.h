@@ -477,9 +477,9 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
  * down[a]: rank x dim, up[a]: out_dim x rank, each contiguous, adapters down_stride / up_stride
  * elements apart -- so a row of an adapter table looked up through the cache can hold both, and the
  * `inverse` of ugc_lookup_unique is the plan's ids.  scale: fp32 per adapter, or NULL for 1.
- * out may be base itself (same stride); other overlaps are not allowed.  fp16 and bf16, rank at most
- * UGC_ADAPTER_MAX_RANK; 16-byte aligned addresses and strides, dims and ranks in multiples of 8
- * elements take the fast loads.  Sums are fp32; the rank products enter the second product as two
+ * out may be base itself (same stride); other overlaps are not allowed.  Rank at most
+ * UGC_ADAPTER_MAX_RANK.  fp16 and bf16 run on the matrix units (fp32 does not, and is many times slower): 16-byte aligned addresses and strides, dims and ranks in multiples of 8
+ * elements take the fast loads.  Sums are fp32; their rank products enter the second product as two
  * 16-bit terms (16 significand bits or more); infinities in an adapter that a token uses may come out as
  * NaN.  workspace: ugc_adapter_workspace bytes (0 for small
  * batches, then NULL will do), 16-byte aligned, free again when the call's work is done. */

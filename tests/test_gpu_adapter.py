@@ -1,16 +1,16 @@
 """Low-rank adapters against the formula in 64 bits.
 
-Bound: the first product's sum of dim terms is off by at most dim * 2^-23 of the sum of its magnitudes (products of
+Bound: the first product's sum of dim terms (and of the 16 partial sums or fewer that it is cut into) is off by at most (dim + 16) * 2^-23 of the sum of its magnitudes (products of
 16-bit values are exact in fp32; an addition inside a matrix instruction may truncate, 2^-23), the scale by 2^-24, the two 16-bit terms by 2^-16 of the
 value (2^-8 of 2^-8) and, below the type's normal range, 2^-24 of the token's largest one; the second sum of 2 * rank terms by
-2 * rank * 2^-23 of its magnitudes, the result by eps / 2."""
+2 * rank * 2^-23 of its magnitudes, the result by eps / 2.  fp32: fused multiply-adds, so 2^-24 for 2^-23, and no terms."""
 import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
 @pytest.fixture(scope="module")
@@ -23,6 +23,9 @@ def formula(base, x, down, up, ids, scale):
     """(result, bound) in 64 bits, adapter by adapter."""
     want, slack = base.double(), torch.zeros_like(base, dtype=torch.float64)
     rank, dim = down.shape[1], down.shape[2]
+    f = torch.finfo(base.dtype)
+    full = base.dtype == torch.float32          # fused multiply-adds, no terms of 16 bits
+    add, term, least, sums = (2.0 ** -24, 0.0, 0.0, rank) if full else (2.0 ** -23, 2.0 ** -16, 2.0 ** -24, 2 * rank)
     for a in range(down.shape[0]):
         t = torch.nonzero(ids == a).reshape(-1)
         if not t.numel():
@@ -30,12 +33,11 @@ def formula(base, x, down, up, ids, scale):
         s = 1.0 if scale is None else float(scale[a].double())
         d, u = down[a].double(), up[a].double()
         inner = x[t].double() @ d.t() * s
-        off = (dim * 2.0 ** -23 + 2.0 ** -24) * (x[t].double().abs() @ d.abs().t()) * abs(s)
-        off = off + 2.0 ** -16 * inner.abs() + 2.0 ** -24 * inner.abs().amax(1, keepdim=True)
+        off = ((dim + 16) * add + 2.0 ** -24) * (x[t].double().abs() @ d.abs().t()) * abs(s)
+        off = off + term * inner.abs() + least * inner.abs().amax(1, keepdim=True)
         want[t] += inner @ u.t()
-        slack[t] += off @ u.abs().t() + 2 * rank * 2.0 ** -23 * ((inner.abs() + off) @ u.abs().t())
-    f = torch.finfo(base.dtype)
-    slack = slack + f.eps / 2 * (want.abs() + slack) + 2.0 ** -23 * (want.abs() + slack) + f.smallest_normal * f.eps / 2
+        slack[t] += off @ u.abs().t() + sums * add * ((inner.abs() + off) @ u.abs().t())
+    slack = slack + f.eps / 2 * (want.abs() + slack) + (0.0 if full else add) * (want.abs() + slack) + f.smallest_normal * f.eps / 2
     return want, slack
 
 
@@ -217,7 +219,7 @@ def test_refusals(rt):
             (lambda: rt.adapter_add(b, x, d[:, :, :32], u, p), ValueError), (lambda: rt.adapter_add(b, x, d[:, :4], u, p), ValueError),
             (lambda: rt.adapter_add(b, x, d[:2], u[:2], p), ValueError), (lambda: rt.adapter_add(b, x, d, u, p, scale=torch.ones(2, device="cuda")), ValueError),
             (lambda: rt.adapter_add(b, x, d, u, p, scale=torch.ones(3, device="cuda").half()), TypeError),
-            (lambda: rt.adapter_add(b.float(), x.float(), d.float(), u.float(), p), rt.UgcError),
+            (lambda: rt.adapter_add(b.double(), x.double(), d.double(), u.double(), p), TypeError),
             (lambda: rt.adapter_add(b, x, torch.zeros(3, 136, 64, dtype=b.dtype, device="cuda"), torch.zeros(3, 32, 136, dtype=b.dtype, device="cuda"), p), rt.UgcError),
             (lambda: rt.adapter_add(b, x, d, u, p, out=b[:, :16]), ValueError)):
         with pytest.raises(error):

@@ -74,7 +74,7 @@ def adapter(L, elem=2, base=A, base_stride=8, x=A, x_stride=16, down=A, down_str
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(elem=0), UNSUPPORTED), (dict(elem=7), INVALID), (dict(rank=0), INVALID), (dict(rank=129), UNSUPPORTED),
+    (dict(elem=3), INVALID), (dict(elem=7), INVALID), (dict(rank=0), INVALID), (dict(rank=129), UNSUPPORTED),
     (dict(dim=0), INVALID), (dict(out_dim=0), INVALID), (dict(groups=0), INVALID), (dict(groups=1025), INVALID),
     (dict(tokens=(1 << 28) + 1), INVALID), (dict(base=None), INVALID), (dict(x=A + 1), INVALID), (dict(x_stride=15), INVALID),
     (dict(base_stride=7), INVALID), (dict(out=None), INVALID), (dict(down=None), INVALID), (dict(down_stride=63), INVALID),

@@ -439,6 +439,95 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 }
 
 // ------------------------------------------------------------------------------------
+// fp32 adapters
+// ------------------------------------------------------------------------------------
+// The matrix units have no fp32 products, so these are fused multiply-adds, 16 tokens a cluster as above: x goes
+// through shared memory 256 columns at a time, a warp has a rank and all tokens; then a thread has an output and all
+// tokens.  For exactness, not for speed: 48 tokens of 64 adapters of rank 16 (4096 x 4096) take 29 us, 16 MB of matrices.
+
+constexpr int kF32Columns = 256;
+
+__global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
+  extern __shared__ __align__(16) float fsmem[];
+  float* part = fsmem;                                             // [token][rank]
+  float* inner = part + kTile * kAdapterMaxRank;                   // [rank][token]
+  float (*columns)[kF32Columns] = reinterpret_cast<float (*)[kF32Columns]>(inner + kTile * kAdapterMaxRank);  // [token]
+  __shared__ int32_t token[kTile];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t member = cluster.block_rank(), members = cluster.num_blocks();
+  const Tile tile = find_tile<kTile, kBlock>(p.offsets, p.n_groups, p.n_tokens, blockIdx.x / members);
+  if (tile.count == 0) return;  // of the whole cluster
+  if (threadIdx.x < kTile) {
+    const uint32_t t = threadIdx.x < tile.count ? (uint32_t)p.order[tile.first + threadIdx.x] : kFull;
+    token[threadIdx.x] = t < p.n_tokens ? (int32_t)t : -1;
+  }
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = p.rank;
+  const float* base = static_cast<const float*>(p.base);
+  float* out = static_cast<float*>(p.out);
+  const bool bare = tile.group == p.n_groups;
+  if (bare && out == base) return;
+  __syncthreads();
+
+  if (!bare) {
+    const float* down = static_cast<const float*>(p.down) + (long long)tile.group * p.down_stride;
+    const float* x = static_cast<const float*>(p.x);
+    const uint32_t k_slice = (p.dim + members - 1) / members;
+    const uint32_t k_end = min(p.dim, (member + 1) * k_slice);
+    for (uint32_t i = threadIdx.x; i < kTile * rank; i += kBlock) part[i] = 0.f;
+    for (uint32_t k0 = member * k_slice; k0 < k_end; k0 += kF32Columns) {
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < kTile * kF32Columns; i += kBlock) {
+        const uint32_t m = i / kF32Columns, k = k0 + i % kF32Columns;
+        columns[m][i % kF32Columns] = token[m] >= 0 && k < k_end ? x[(long long)token[m] * p.x_stride + k] : 0.f;
+      }
+      __syncthreads();
+      for (uint32_t r = warp; r < rank; r += kWarps) {
+        float acc[kTile] = {};
+#pragma unroll
+        for (int c = 0; c < kF32Columns / 32; c++) {
+          const uint32_t k = k0 + c * 32 + lane;
+          const float d = k < k_end ? down[(size_t)r * p.dim + k] : 0.f;
+#pragma unroll
+          for (int m = 0; m < kTile; m++) acc[m] = fmaf(columns[m][c * 32 + lane], d, acc[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < kTile; m++) {
+#pragma unroll
+          for (int d = 16; d; d >>= 1) acc[m] += __shfl_xor_sync(kFull, acc[m], d);
+          if (lane == 0) part[m * rank + r] += acc[m];
+        }
+      }
+    }
+    cluster_arrive();
+    cluster_wait();
+    const float scale = p.scale ? p.scale[tile.group] : 1.f;
+    for (uint32_t i = threadIdx.x; i < kTile * rank; i += kBlock) {  // the CTAs' sums, in their order
+      float sum = 0.f;
+      for (uint32_t w = 0; w < members; w++) sum += cluster.map_shared_rank(part, w)[i];
+      inner[i % rank * kTile + i / rank] = sum * scale;
+    }
+    __syncthreads();
+    cluster_arrive();  // waited for at the end: nobody leaves while its sums are being read
+  }
+  const uint32_t n_slice = (p.out_dim + members - 1) / members, n_end = min(p.out_dim, (member + 1) * n_slice);
+  const float* up = static_cast<const float*>(p.up) + (bare ? 0 : (long long)tile.group * p.up_stride);
+  for (uint32_t n = member * n_slice + threadIdx.x; n < n_end; n += kBlock) {
+    float acc[kTile] = {};
+    for (uint32_t r = 0; !bare && r < rank; r++) {
+      const float u = up[(size_t)n * rank + r];
+#pragma unroll
+      for (int m = 0; m < kTile; m++) acc[m] = fmaf(inner[r * kTile + m], u, acc[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < kTile; m++)
+      if (token[m] >= 0) out[(long long)token[m] * p.out_stride + n] = base[(long long)token[m] * p.base_stride + n] + acc[m];
+  }
+  if (!bare) cluster_wait();
+}
+
+// ------------------------------------------------------------------------------------
 // prompts: tiles of 128 tokens on the 5th-generation tensor cores
 // ------------------------------------------------------------------------------------
 // Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
@@ -978,27 +1067,17 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   if (warp == 12) free_tensor_memory<kColumns>(tmem);
 }
 
-template <typename E, int RP>
-cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t stream) {
-  using S = SmallShape<RP>;
-  auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
-  constexpr uint32_t kSms = 148;
-  const uint32_t tiles = p.n_tokens / kTile + std::min(p.n_groups + 1, p.n_tokens);
-  // Clusters of 8 are the shorter chain, of 4 the less work a tile: 64 tiles of rank 16 (4096 x 4096) 10.7 against 13.3 us,
-  // 128 tiles 15.6 against 12.8.
-  const bool few = tiles * kMostCluster <= kSms * 9 / 2;
-  const uint32_t cluster = few ? kMostCluster : kMostCluster / 2;
-  // CTAs an SM, by shared memory: as few as hold the batch, so that they spread over all SMs (packed onto few
-  // of them 30 tiles took 9.9 us instead of 8.5), and of small clusters at most three (mixed prompts of 200 adapters 18.7 us
-  // with four, 16.4 with three).  What is left of it holds `up`.
-  constexpr uint32_t kMost = RP <= 32 ? 3 : 2;
-  const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, few && RP <= 16 ? 4 : kMost);
-  const uint32_t budget = std::min(216u * 1024 / per_sm, 200u * 1024);
-  const uint32_t slice = (p.out_dim + cluster * 32 - 1) / (cluster * 32) * 32;
-  const uint32_t room = vector ? (uint32_t)std::min<size_t>(budget - S::kShared, (size_t)slice * p.rank * 2) / 16 * 16 : 0;
-  const size_t smem = budget;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+// Tiles of 16 tokens, at most: every group may end in one of its own.
+uint32_t small_tiles(const AdapterParams& p) { return p.n_tokens / kTile + std::min(p.n_groups + 1, p.n_tokens); }
+
+// A cluster of CTAs a tile.
+template <typename... KArgs, typename... Args>
+cudaError_t cluster_launch(void (*kern)(KArgs...), uint32_t tiles, uint32_t cluster, size_t smem, cudaStream_t stream,
+                           const Args&... args) {
+  if (smem > 47 * 1024) {  // beside what is static
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * cluster);
   cfg.blockDim = dim3(kBlock);
@@ -1011,7 +1090,28 @@ cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t str
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, p, room);
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <typename E, int RP>
+cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t stream) {
+  using S = SmallShape<RP>;
+  auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
+  constexpr uint32_t kSms = 148;
+  const uint32_t tiles = small_tiles(p);
+  // Clusters of 8 are the shorter chain, of 4 the less work a tile: 64 tiles of rank 16 (4096 x 4096) 10.7 against 13.3 us,
+  // 128 tiles 15.6 against 12.8.
+  const bool few = tiles * kMostCluster <= kSms * 9 / 2;
+  const uint32_t cluster = few ? kMostCluster : kMostCluster / 2;
+  // CTAs an SM, by shared memory: as few as hold the batch, so that they spread over all SMs (packed onto few
+  // of them 30 tiles took 9.9 us instead of 8.5), and of small clusters at most three (mixed prompts of 200 adapters 18.7 us
+  // with four, 16.4 with three).  What is left of it holds `up`.
+  constexpr uint32_t kMost = RP <= 32 ? 3 : 2;
+  const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, few && RP <= 16 ? 4 : kMost);
+  const uint32_t budget = std::min(216u * 1024 / per_sm, 200u * 1024);
+  const uint32_t slice = (p.out_dim + cluster * 32 - 1) / (cluster * 32) * 32;
+  const uint32_t room = vector ? (uint32_t)std::min<size_t>(budget - S::kShared, (size_t)slice * p.rank * 2) / 16 * 16 : 0;
+  return cluster_launch(kern, tiles, cluster, budget, stream, p, room);
 }
 
 int padded_rank(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
@@ -1085,6 +1185,10 @@ cudaError_t adapter_stalled(uint32_t* count) { return cudaMemcpyFromSymbol(count
 
 cudaError_t launch_adapter_add(const AdapterParams& p, int elem, void* scratch, cudaStream_t stream) {
   if (p.n_tokens == 0) return cudaSuccess;
+  if (elem == kElemF32) {
+    const size_t smem = (2 * kTile * kAdapterMaxRank + kTile * kF32Columns) * sizeof(float);
+    return cluster_launch(adapter_f32_kernel, small_tiles(p), kMostCluster, smem, stream, p);
+  }
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(p.base) | reinterpret_cast<uintptr_t>(p.x) |
                               reinterpret_cast<uintptr_t>(p.down) | reinterpret_cast<uintptr_t>(p.up) |
                               reinterpret_cast<uintptr_t>(p.out);

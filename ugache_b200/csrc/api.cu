@@ -2881,8 +2881,8 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
                     size_t out_dim, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
   size_t need = 0;
   UGC_TRY(ugc_adapter_workspace(n_tokens, n_groups, rank, dim, out_dim, &need));
-  if (elem_type == UGC_ELEM_F32) return fail(UGC_ERR_UNSUPPORTED, "adapters are fp16 or bf16");
-  if (elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16) return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
+  if (elem_type != UGC_ELEM_F32 && elem_type != UGC_ELEM_F16 && elem_type != UGC_ELEM_BF16)
+    return fail(UGC_ERR_INVALID, "unknown element type %d", elem_type);
   if (n_tokens == 0) return UGC_OK;
   UGC_TRY(check_rows("base", base, base_stride, out_dim, elem_type));
   UGC_TRY(check_rows("out", out, out_stride, out_dim, elem_type));
