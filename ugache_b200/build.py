@@ -20,7 +20,7 @@ FAST_STAMP = os.path.join(HERE, "build", "fast_stamp.txt")
 CUDA_SOURCES = ["kernels.cu", "routing.cu", "adapter.cu", "api.cu"]
 HOST_SOURCES = ["placement.cc", "compat_api.cc"]
 FAST_SOURCE = "pyfast.cc"
-HEADERS = ["device_types.h", "kernels.cuh", "routing.cuh", "placement.h", "../../include/ugache_b200.h",
+HEADERS = ["device_types.h", "kernels.cuh", "routing.cuh", "lanes.cuh", "placement.h", "../../include/ugache_b200.h",
            "../../include/coll_cache_api.h", "../../include/coll_cache_lib/facade.h"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,6 +1,8 @@
 // Low-rank adapters of many requests at once: out[t] = base[t] + scale[a] * (x[t] down[a]^T) up[a]^T.
 #include "routing.cuh"
 
+#include "lanes.cuh"
+
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -14,7 +16,6 @@ namespace ugc {
 
 namespace {
 
-constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kBlock = kWarps * 32;
 constexpr int kTile = 16;     // tokens of a tile: the rows of one matrix instruction
@@ -159,12 +160,10 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
 // the cluster has a slice of dim and, later, of out_dim; the CTAs hand one another their partial rank products
 // through distributed shared memory.  `up` does not wait for those: a bulk copy brings the slice
 // (what fits) into shared memory meanwhile.  The matrix instructions take the columns of a product in any
-// order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.
+// order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.  4096 x 4096, bf16: one token of
+// rank 16 6.7 us, 48 tokens of 64 adapters 8.6 us (8.1 MB of matrices), of rank 64 15 us, of rank 128 30 us (66 MB, 2.2 TB/s).
 
 constexpr int kMostCluster = 8;
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Columns [begin, end) of the rows of a tile's tokens from one matrix to another; by THREADS threads, four pieces each in
 // flight.  token(m): the m-th token of the tile, negative for none.
@@ -443,7 +442,8 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 // ------------------------------------------------------------------------------------
 // The matrix units have no fp32 products, so these are fused multiply-adds, 16 tokens a cluster as above: x goes
 // through shared memory 256 columns at a time, a warp has a rank and all tokens; then a thread has an output and all
-// tokens.  For exactness, not for speed: 48 tokens of 64 adapters of rank 16 (4096 x 4096) take 29 us, 16 MB of matrices.
+// tokens.  Bound by its instructions: 48 tokens of 64 adapters of rank 16 (4096 x 4096) take 28 us, 16,384 of 24 of
+// rank 64 1.56 ms (17 GFLOP; 3.2 ms with every sum shuffled alone and `up` read an element at a time).
 
 constexpr int kF32Columns = 256;
 
@@ -492,12 +492,9 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
 #pragma unroll
           for (int m = 0; m < kTile; m++) acc[m] = fmaf(columns[m][c * 32 + lane], d, acc[m]);
         }
-#pragma unroll
-        for (int m = 0; m < kTile; m++) {
-#pragma unroll
-          for (int d = 16; d; d >>= 1) acc[m] += __shfl_xor_sync(kFull, acc[m], d);
-          if (lane == 0) part[m * rank + r] += acc[m];
-        }
+        uint32_t m;
+        const float sum = sum_over_lanes(acc, 32, &m);
+        if ((lane & (32 / kTile - 1)) == 0) part[m * rank + r] += sum;
       }
     }
     cluster_arrive();
@@ -513,12 +510,29 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
   }
   const uint32_t n_slice = (p.out_dim + members - 1) / members, n_end = min(p.out_dim, (member + 1) * n_slice);
   const float* up = static_cast<const float*>(p.up) + (bare ? 0 : (long long)tile.group * p.up_stride);
+  const bool vector = rank % 4 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0;
   for (uint32_t n = member * n_slice + threadIdx.x; n < n_end; n += kBlock) {
     float acc[kTile] = {};
-    for (uint32_t r = 0; !bare && r < rank; r++) {
-      const float u = up[(size_t)n * rank + r];
+    for (uint32_t r = 0; !bare && r < rank; r += 4) {
+      float u[4] = {};
+      if (vector) {
+        const float4 v = *reinterpret_cast<const float4*>(up + (size_t)n * rank + r);
+        u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+      } else {
 #pragma unroll
-      for (int m = 0; m < kTile; m++) acc[m] = fmaf(inner[r * kTile + m], u, acc[m]);
+        for (int i = 0; i < 4; i++)
+          if (r + i < rank) u[i] = up[(size_t)n * rank + r + i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (r + i >= rank) break;  // what lies behind the last rank in shared memory is no product
+#pragma unroll
+        for (int m = 0; m < kTile; m += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(inner + (r + i) * kTile + m);
+          acc[m] = fmaf(x.x, u[i], acc[m]), acc[m + 1] = fmaf(x.y, u[i], acc[m + 1]);
+          acc[m + 2] = fmaf(x.z, u[i], acc[m + 2]), acc[m + 3] = fmaf(x.w, u[i], acc[m + 3]);
+        }
+      }
     }
 #pragma unroll
     for (int m = 0; m < kTile; m++)
@@ -538,7 +552,9 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
 // of the first product, the tile has one more partial sum.
 // Steps go through a ring of stages in shared memory: four warps copy (token rows lie anywhere, so 16
 // bytes a thread), one thread issues the matrix instructions, the other warps take the products out of
-// tensor memory.
+// tensor memory.  HBM bounds it, through the bytes that the ring keeps in flight: 4096 x 4096, bf16, 16,384 tokens of 24
+// adapters of rank 16 / 64 / 128 take 80 / 89 / 119 us (62 / 65 / 69 at the rate of a plain copy), 65,536 of rank 64
+// 305 (250); with two stages less 90 at rank 16.
 //
 // Operands lie in shared memory in rows of 128 bytes whose 16-byte pieces are exchanged by row (piece c
 // of row r at c ^ (r % 8)), as the matrix unit reads them: a line of global memory is a line there, and

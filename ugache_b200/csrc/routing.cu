@@ -2,6 +2,8 @@
 // and back, weighted, with the inner products that the weights' gradients are.
 #include "routing.cuh"
 
+#include "lanes.cuh"
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -12,13 +14,9 @@ namespace ugc {
 
 namespace {
 
-constexpr unsigned kFull = 0xffffffffu;
-
 __device__ __forceinline__ void wait_for_launch_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_launch_behind() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // A word of shared memory as CTA `rank` of the cluster has it at the same place.
 __device__ __forceinline__ uint32_t count_of(const uint32_t* mine, uint32_t rank) {
   uint32_t at, v;
@@ -306,7 +304,8 @@ struct PlanShape {
   Shared shared;
   uint32_t parts, part, block;
 };
-// 1024 ids take 4.1 us in one CTA, 8192 12 us; in a cluster of eight the latter take 5, 65,536 ids 10.
+// On the GPU: 256 ids 2.5 us and 1024 4.1 in one CTA; 8192 took 12 there and take 6.3 in a cluster of eight, 65,536 ids
+// 11; 524,288 12.8 in parts, a million 18.6.
 PlanShape plan_shape(uint32_t n) {
   auto up_to = [](uint32_t v, uint32_t a) { return (v + a - 1) / a * a; };
   PlanShape s{Shared::kNot, 1, n, 128};
@@ -458,7 +457,8 @@ __global__ void __launch_bounds__(kRowsBlock) spread_kernel(RouteRows p, uint32_
 }
 
 // A thread sums PIECES pieces of one token's row over its choices, in their order, in fp32: FLIGHT choices and
-// all pieces are on their way at once.
+// all pieces are on their way at once.  Bound by the bytes in flight: 32,768 tokens of 4 rows of 8 KiB 213 us (6.3 TB/s) with
+// 4 x 2, 249 with 4 x 1, 292 with 4 x 4 (registers); two rows of 32 KiB 120 us with 2 x 4, 167 with 4 x 1.
 template <typename E, bool WEIGHTED, int FLIGHT, int PIECES>
 __global__ void __launch_bounds__(kRowsBlock) gather_kernel(RouteRows p, uint32_t pieces) {
   wait_for_launch_ahead();
@@ -500,31 +500,6 @@ __global__ void __launch_bounds__(kRowsBlock) gather_kernel(RouteRows p, uint32_
   for (int i = 0; i < PIECES; i++) st_piece(row_at(p.token_out, p.token_out_stride, t), c + i * stride, sum[i].rounded());
 }
 
-// The sums of N (a power of two) values of each lane over `width` (N to 32) lanes: at every step a lane keeps half
-// of its values and hands over the others, so that it takes N - 1 + log2(width / N) exchanges instead of N * log2(width).
-// The order of the additions is the same wherever a value ends.  Returns the sum of value `which`.
-template <int N>
-__device__ __forceinline__ float sum_over_lanes(float (&v)[N], uint32_t width, uint32_t* which) {
-  const uint32_t lane = threadIdx.x & 31;
-  uint32_t at = 0;
-  int n = N, d = (int)width / 2;
-#pragma unroll
-  for (int step = N; step > 1; step >>= 1, d >>= 1) {
-    n = step / 2;
-    const bool upper = lane & d;
-#pragma unroll
-    for (int i = 0; i < N / 2; i++)
-      if (i < n) {
-        const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
-        v[i] = keep + __shfl_xor_sync(kFull, give, d);
-      }
-    if (upper) at += n;
-  }
-  for (; d; d >>= 1) v[0] += __shfl_xor_sync(kFull, v[0], d);
-  *which = at;
-  return v[0];
-}
-
 // The lanes' sums of N choices' products into the dots: by the whole CTA.
 template <int N>
 __device__ __forceinline__ void share_sums(float (&dot)[N], float (*share)[N], const RouteRows& p, size_t at, uint32_t j0,
@@ -557,7 +532,8 @@ __device__ __forceinline__ void share_sums(float (&dot)[N], float (*share)[N], c
 
 // Inner products of a token's row with the rows of its choices, and the spread or the gather on the way: `lanes`
 // threads (a power of two, fixed by the row's length, so that results do not depend on the batch) walk the row
-// together.  All rows' pieces are loaded before anything is stored.
+// together.  All rows' pieces are loaded before anything is stored.  16,384 tokens of 6 rows of 4 KiB 145 us (216 with
+// loads and stores in turn), of 8 gathered 117 us; bound by HBM, reads and writes mixed.
 template <typename E, bool WEIGHTED, bool SPREAD, int CHOICES>
 __global__ void __launch_bounds__(kRowsBlock, 2) dots_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
   wait_for_launch_ahead();
