@@ -68,8 +68,8 @@ __device__ __forceinline__ uint32_t group_of(IdT id, uint32_t n_groups) {
   return (unsigned long long)(long long)id < n_groups ? (uint32_t)id : n_groups;  // one more group: no group
 }
 
-// The lanes whose id is in the same group, bit by bit of the group (a match instruction takes several times as
-// long: 8192 ids in one CTA 13.7 us).  Meant for lanes that are `live`.
+// The lanes whose id is in the same group, bit by bit of the group (8192 ids in one CTA took 13.7 us with a match
+// instruction, 12.1 with this).  Meant for lanes that are `live`.
 __device__ __forceinline__ unsigned lanes_of_group(uint32_t group, bool live, uint32_t bits) {
   unsigned same = __ballot_sync(kFull, live);
 #pragma unroll 4
