@@ -161,7 +161,8 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
 // through distributed shared memory.  `up` does not wait for those: a bulk copy brings the slice
 // (what fits) into shared memory meanwhile.  The matrix instructions take the columns of a product in any
 // order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.  4096 x 4096, bf16: one token of
-// rank 16 6.7 us, 48 tokens of 64 adapters 8.6 us (8.1 MB of matrices), of rank 64 15 us, of rank 128 30 us (66 MB, 2.2 TB/s).
+// rank 16 6.1 us (2.1 until its tile is known, 1.0 for the first product, 1.6 for the cluster's sums, 1.4 for the second), 48
+// tokens of 64 adapters 7.7 us (8.1 MB of matrices), of rank 64 15 us, of rank 128 31 us (66 MB, 2.1 TB/s).
 
 constexpr int kMostCluster = 8;
 
@@ -317,28 +318,29 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
     }
   }
   cluster_arrive();
-  uint32_t in[2][4] = {};  // base of the warp's next columns
-  auto load_base = [&](uint32_t n0) {
+  uint32_t in[2][2][4] = {};  // base of the warp's next two runs of columns
+  auto load_base = [&](uint32_t (&to)[2][4], uint32_t n0) {
 #pragma unroll
     for (int o = 0; o < 2; o++) {
       const int t = token[g + 8 * o], at = (int)(n0 + c * 8), valid = (int)n_end - at;
-      if (t >= 0 && valid > 0) load_words<4, VECTOR>(in[o], base + (long long)t * p.base_stride + at, valid);
+      if (t >= 0 && valid > 0) load_words<4, VECTOR>(to[o], base + (long long)t * p.base_stride + at, valid);
     }
   };
-  load_base(n_begin + warp * 32);
+  load_base(in[0], n_begin + warp * 32);
+  load_base(in[1], n_begin + warp * 32 + kWarps * 32);
   cluster_wait();
   // the CTAs' sums, in their order; scaled to the token's largest so that both 16-bit terms keep their bits
   {
     const float scale = p.scale ? p.scale[tile.group] : 1.f;
     constexpr int kRounds = (KR + 63) / 64;
-    for (uint32_t m = warp; m < kTile; m += kWarps) {
+    for (uint32_t m = warp; m < tile.count; m += kWarps) {  // rows behind stay as they are: their products are not stored
       float2 u[kRounds];
       float top = 0.f;
 #pragma unroll
       for (int o = 0; o < kRounds; o++) {
         const uint32_t r = o * 64 + lane * 2;
         u[o] = make_float2(0.f, 0.f);
-        if (m < tile.count && r < RP) {
+        if (r < RP) {
           float2 v[kMostCluster];
 #pragma unroll
           for (int w = 0; w < kMostCluster; w++)
@@ -392,18 +394,25 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 #pragma unroll
       for (int o = 0; o < 2; o++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[o][i] = in[o][i];
-      load_base(n0 + kWarps * 32);
+        for (int i = 0; i < 4; i++) {
+          y[o][i] = in[0][o][i];
+          in[0][o][i] = in[1][o][i];
+        }
+      load_base(in[1], n0 + 2 * kWarps * 32);
+      const bool here = n0 - n_begin + 32 <= held;  // all of the run's rows of `up` are in shared memory
       float acc[4][4] = {};
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const uint32_t n = n0 + (g >> 1) * 8 + q * 2 + (g & 1);
-        const uint16_t* row = n - n_begin < held ? up_here + (size_t)(n - n_begin) * p.rank : up + (size_t)n * p.rank;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           uint32_t b[W] = {};
           const int r = (s * 4 + (int)c) * 2 * W, left = (int)p.rank - r;
-          if (n < n_end && left > 0) load_words<W, VECTOR>(b, row + r, left);
+          if (here) {
+            if (left > 0) load_words<W, VECTOR>(b, up_here + (n - n_begin) * p.rank + r, left);
+          } else if (n < n_end && left > 0) {
+            load_words<W, VECTOR>(b, up + (size_t)n * p.rank + r, left);
+          }
 #pragma unroll
           for (int h = 0; h < 2; h++)
 #pragma unroll
