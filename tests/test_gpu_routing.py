@@ -47,6 +47,13 @@ def test_plan(rt, n, G):
     check_plan(rt, ids, G, torch.int64 if n % 2 else torch.int32)
 
 
+# shared memory of a CTA on both sides of what a launch gets without asking
+@pytest.mark.parametrize("n", [30000, 36000, 40000, 42000, 44000, 46000, 48000, 50000])
+@pytest.mark.parametrize("G", [1, 256, 500, 700])
+def test_plan_shared_memory(rt, n, G):
+    check_plan(rt, np.random.default_rng(n).integers(0, G, n), G)
+
+
 @pytest.mark.parametrize("shape", [(5, 3), (4096, 8), (1, 1), (0, 4), (17, 20)])
 def test_plan_shapes(rt, shape):
     check_plan(rt, np.random.default_rng(1).integers(0, 12, shape), 12)

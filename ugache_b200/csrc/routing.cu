@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t count_of(const uint32_t* mine, uint32_t rank
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, bool pdl,
                    unsigned cluster, const Args&... args) {
-  if (smem > 48 * 1024) {
+  if (smem > 36 * 1024) {  // with what is static (up to 9 KB) beyond the 48 KB that need no word
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
