@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -109,19 +110,18 @@ def build(force=False, verbose=False):
 def _build_library():
     nvcc = _nvcc()
     bdir = os.path.join(HERE, "build")
-    objs = []
-    log = []
-    for src in CUDA_SOURCES + HOST_SOURCES:
-        path = os.path.join(CSRC, src)
-        if not os.path.exists(path):
-            continue
-        obj = os.path.join(bdir, os.path.splitext(src)[0] + ".o")
-        cmd = [nvcc] + NVCC_FLAGS + ["-c", path, "-o", obj]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        log.append(r.stderr)
+    sources = [src for src in CUDA_SOURCES + HOST_SOURCES if os.path.exists(os.path.join(CSRC, src))]
+    objs = [os.path.join(bdir, os.path.splitext(src)[0] + ".o") for src in sources]
+
+    def compile_one(src, obj):
+        return subprocess.run([nvcc] + NVCC_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj], capture_output=True, text=True)
+
+    with ThreadPoolExecutor(len(sources) or 1) as pool:  # one compiler a source
+        results = list(pool.map(compile_one, sources, objs))
+    log = [r.stderr for r in results]
+    for src, r in zip(sources, results):
         if r.returncode != 0:
             raise RuntimeError("nvcc failed on %s:\n%s" % (src, r.stderr))
-        objs.append(obj)
     cmd = [nvcc, "-shared", "-o", LIB] + objs + ["-cudart", "static", "-Xcompiler", "-fopenmp",
                                                   "-gencode", "arch=compute_100a,code=sm_100a"]
     r = subprocess.run(cmd, capture_output=True, text=True)
