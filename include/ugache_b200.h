@@ -479,9 +479,9 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
  * `inverse` of ugc_lookup_unique is the plan's ids.  scale: fp32 per adapter, or NULL for 1.
  * out may be base itself (same stride); other overlaps are not allowed.  Rank at most
  * UGC_ADAPTER_MAX_RANK.  fp16 and bf16 run on the matrix units (fp32 does not, and is many times slower): 16-byte aligned addresses and strides, dims and ranks in multiples of 8
- * elements take the fast loads.  Sums are fp32; their rank products enter the second product as two
- * 16-bit terms (16 significand bits or more); infinities in an adapter that a token uses may come out as
- * NaN.  workspace: ugc_adapter_workspace bytes (0 for small
+ * elements take the fast loads.  Sums are fp32; the rank products enter the second product as three
+ * 16-bit terms, which hold all 24 bits of the sum (fp16: of those down to 2^-16 of the token's largest,
+ * below that 2^-39 of the largest); infinities in an adapter that a token uses may come out as NaN.  workspace: ugc_adapter_workspace bytes (0 for small
  * batches, then NULL will do), 16-byte aligned, free again when the call's work is done. */
 #define UGC_ADAPTER_MAX_RANK 128
 int ugc_adapter_workspace(size_t n_tokens, int n_groups, size_t rank, size_t dim, size_t out_dim, size_t* bytes);

@@ -1,0 +1,74 @@
+"""What the rank products of 16-bit adapters keep between the two products: 24 significand bits, as an fp32 sum has.
+
+Inputs are chosen so that both sums are exact in fp32 (whole numbers below 2^24, or one term a sum), so that what is
+left is the way the rank products are handed over and the result's one rounding."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def rt(built_lib):
+    from ugache_b200 import runtime
+    return runtime
+
+
+def run(rt, base, x, down, up, ids, **kw):
+    return rt.adapter_add(base, x, down, up, rt.route_plan(ids, down.shape[0]), **kw)
+
+
+@pytest.mark.parametrize("rank", [8, 16, 24, 64, 72, 128])
+@pytest.mark.parametrize("T", [50, 6000])   # single tokens, prompts
+def test_whole_numbers_are_exact(rt, rank, T):
+    """Rank products of 18 to 20 bits; `base` takes away all that the result's type could hide."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T + rank)
+    G, dim, out_dim = 3, 64, 136
+
+    def whole(low, high, *size):
+        return torch.randint(low, high + 1, size, generator=g, device="cuda")
+
+    x, down = whole(0, 127, T, dim), whole(0, 127, G, rank, dim)       # sums up to 64 * 127^2 < 2^20
+    up = torch.zeros((G, out_dim, rank), dtype=torch.int64, device="cuda")
+    for _ in range(4):                                                 # at most four ranks an output, each at most 3 in the end
+        up.scatter_(2, whole(0, rank - 1, G, out_dim, 1), whole(-1, 1, G, out_dim, 1))
+    ids = whole(0, G - 1, T)
+    delta = torch.einsum("tr,tnr->tn", torch.einsum("td,trd->tr", x.double(), down[ids].double()), up[ids].double())
+    assert float(delta.abs().max()) < 2 ** 23
+    ty = torch.bfloat16
+    base = (-delta).to(ty)
+    got = run(rt, base, x.to(ty), down.to(ty), up.to(ty), ids)
+    want = (base.double() + delta).to(ty)
+    assert bool((want != 0).any()) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("elem", sorted(TYPES))
+@pytest.mark.parametrize("rank", [8, 16, 24, 64, 128])
+@pytest.mark.parametrize("T", [50, 6000])
+def test_ranks_of_far_magnitudes(rt, rank, T, elem):
+    """Rank product r of a token is m * 2^-e(r), m of up to 11 bits in [1, 2) and e from 0 to 20; output n takes one rank
+    alone and scales it back.  Two roundings: a rank product's to 24 bits (2^-23 of it, whatever cuts them off; or 2^-38 of the
+    token's largest, 2, where the type ends below it) and the result's, by eps / 2."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T + 3 * rank)
+    G, ty = 2, TYPES[elem]
+    dim = out_dim = max(rank, 16)
+    e = (torch.arange(rank, device="cuda") * 7) % 21
+    m = (1 + torch.rand((T, dim), generator=g, device="cuda")).to(ty)
+    down = torch.zeros((G, rank, dim), device="cuda")
+    up = torch.zeros((G, out_dim, rank), device="cuda")
+    r = torch.arange(rank, device="cuda")
+    down[:, r, r] = 2.0 ** -e.float()
+    n = torch.arange(out_dim, device="cuda")
+    up[:, n, n % rank] = (2.0 ** e[n % rank].float()).clamp(max=2.0 ** 15)
+    ids = torch.randint(0, G, (T,), generator=g, device="cuda")
+    assert torch.equal(down.to(ty).float(), down) and torch.equal(up.to(ty).float(), up)
+    got = run(rt, torch.zeros((T, out_dim), dtype=ty, device="cuda"), m, down.to(ty), up.to(ty), ids)
+    inner = torch.zeros((T, rank), dtype=torch.float64, device="cuda")
+    inner[:] = m[:, :rank].double() * 2.0 ** -e.double()
+    want = inner @ up[0].double().t()
+    off = (2.0 ** -23 * inner + 2.0 ** -38 * 2) @ up[0].double().t()
+    assert bool(((got.double() - want).abs() <= off + torch.finfo(ty).eps / 2 * (want + off)).all())

@@ -29,6 +29,10 @@ struct Half<__half> {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  // Terms: a token's largest rank product is scaled to [2^14, 2^15), so that what a term leaves of smaller ones is
+  // above the type's last step (2^-24) too: 24 bits of values down to 2^-16 of the largest, 2^-39 of the largest below.
+  static constexpr bool kScaled = true;
+  static __device__ __forceinline__ uint32_t first_bits(float a, float b) { return narrow(a, b); }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -41,6 +45,13 @@ struct Half<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t narrow(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  // Terms: the range is that of fp32, so nothing is scaled; cut off, not rounded, so that none becomes infinite.
+  static constexpr bool kScaled = false;
+  static __device__ __forceinline__ uint32_t first_bits(float a, float b) {
+    uint32_t h;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
+    return h;
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -71,10 +82,26 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint16_t* p, 
   }
 }
 
-// A power of two s with max * s in [1, 2); 1 where there is none.
-__device__ __forceinline__ float unit_scale(float max) {
+// The rank products enter the second product as three 16-bit terms: each takes what the ones before it left, so that
+// together they hold the 24 bits of the fp32 sum (8 + 8 + 8, or 11 + 11 and the rest).
+constexpr int kTerms = 3;
+template <typename E>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&term)[kTerms]) {
+#pragma unroll
+  for (int t = 0; t < kTerms; t++) {
+    term[t] = Half<E>::first_bits(a, b);
+    const float2 h = Half<E>::widen(term[t]);
+    a = t == 0 && isinf(h.x) ? 0.f : a - h.x;  // exact; nothing is left of an infinite value
+    b = t == 0 && isinf(h.y) ? 0.f : b - h.y;
+  }
+}
+
+// The part of a rank product that counts for its token's scale.
+__device__ __forceinline__ float size_of(float v) { return isinf(v) ? 0.f : fabsf(v); }
+// A power of two s, 1 / s one too, with max * s in [2^14, 2^15), or below where max is tiny.
+__device__ __forceinline__ float scale_for(float max) {
   const int e = (int)(__float_as_uint(max) >> 23 & 255) - 127;
-  return max > 0.f && e > -120 && e < 126 ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+  return __uint_as_float((uint32_t)(127 + min(14 - e, 126)) << 23);
 }
 
 // Tile `index` of the batch: tiles of ROWS tokens, group by group, those without a group last.  By the whole CTA.
@@ -203,9 +230,11 @@ struct SmallShape {
   static constexpr int kWarpRanks = RP < 32 ? RP : 32;          // ranks a warp has in the first product
   static constexpr int kRankGroups = RP / kWarpRanks;
   static constexpr int kDepthGroups = kWarps / kRankGroups;     // warps that share a slice of dim
-  static constexpr int kDepth = RP < 16 ? 16 : RP;              // ranks as the second product's depth
+  // the second product's depth; at 8 ranks the first two terms lie side by side in it
+  static constexpr int kDepth = RP < 16 ? 16 : RP;
+  static constexpr int kSlabs = RP < 16 ? 2 : kTerms;
   static constexpr int kPart = kDepthGroups * kTile * RP * 4;
-  static constexpr int kInner = 2 * kTile * (kDepth + 8) * 2;
+  static constexpr int kInner = kSlabs * kTile * (kDepth + 8) * 2;
   static constexpr int kShared = kPart + kInner;                // and what is held of `up`
 };
 
@@ -216,7 +245,7 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   extern __shared__ __align__(128) unsigned char smem[];
   using Inner = uint16_t[kTile][KR + 8];
   float* part = reinterpret_cast<float*>(smem);                              // [depth group][token][rank]
-  Inner* inner = reinterpret_cast<Inner*>(smem + S::kPart);                  // [term]
+  Inner* inner = reinterpret_cast<Inner*>(smem + S::kPart);                  // [slab]
   uint16_t* up_here = reinterpret_cast<uint16_t*>(smem + S::kPart + S::kInner);
   __shared__ float back[kTile];
   __shared__ int32_t token[kTile];
@@ -329,10 +358,10 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   load_base(in[0], n_begin + warp * 32);
   load_base(in[1], n_begin + warp * 32 + kWarps * 32);
   cluster_wait();
-  // the CTAs' sums, in their order; scaled to the token's largest so that both 16-bit terms keep their bits
+  // the CTAs' sums, in their order, and their terms
   {
     const float scale = p.scale ? p.scale[tile.group] : 1.f;
-    constexpr int kRounds = (KR + 63) / 64;
+    constexpr int kRounds = (RP + 63) / 64;
     for (uint32_t m = warp; m < tile.count; m += kWarps) {  // rows behind stay as they are: their products are not stored
       float2 u[kRounds];
       float top = 0.f;
@@ -350,23 +379,25 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
             if (w < members) u[o].x += v[w].x, u[o].y += v[w].y;
           u[o].x *= scale, u[o].y *= scale;
         }
-        top = fmaxf(top, fmaxf(fabsf(u[o].x), fabsf(u[o].y)));
+        top = fmaxf(top, fmaxf(size_of(u[o].x), size_of(u[o].y)));
       }
+      float s = 1.f;
+      if (Half<E>::kScaled) {
 #pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-      const float s = unit_scale(top);
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+        s = scale_for(top);
+      }
       if (lane == 0) back[m] = 1.f / s;
 #pragma unroll
       for (int o = 0; o < kRounds; o++) {
         const uint32_t r = o * 64 + lane * 2;
-        if (r >= KR) continue;
-        const float u0 = u[o].x * s, u1 = u[o].y * s;
-        const uint32_t hi = Half<E>::narrow(u0, u1);
-        const float2 h = Half<E>::widen(hi);
-        // what the first term leaves; nothing where the first is infinite
-        const uint32_t lo = Half<E>::narrow(isinf(h.x) ? 0.f : u0 - h.x, isinf(h.y) ? 0.f : u1 - h.y);
-        *reinterpret_cast<uint32_t*>(&inner[0][m][r]) = hi;
-        *reinterpret_cast<uint32_t*>(&inner[1][m][r]) = lo;
+        if (r >= RP) continue;
+        uint32_t term[kTerms];
+        split<E>(u[o].x * s, u[o].y * s, term);
+#pragma unroll
+        for (int t = 0; t < kTerms; t++)
+          *reinterpret_cast<uint32_t*>(&inner[t * RP / KR][m][t * RP % KR + r]) = term[t];
+        if (RP < KR) *reinterpret_cast<uint32_t*>(&inner[1][m][RP + r]) = 0;
       }
     }
   }
@@ -380,14 +411,17 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   {
     constexpr int KS = KR >= 32 ? KR / 32 : 1;   // steps of 32 (16) ranks
     constexpr int W = KR >= 32 ? 4 : 2;          // words a lane has of one
-    uint32_t u[2][2][KS][W];                     // term, half of the tile
+    constexpr bool kKeep = KS <= 2;              // 96 registers of terms are too many: rank 128 reads them again
+    uint32_t u[kKeep ? KS : 1][S::kSlabs][2][W]; // slab, half of the tile
+    auto load_terms = [&](uint32_t (&to)[S::kSlabs][2][W], int s) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+      for (int h = 0; h < S::kSlabs; h++)
 #pragma unroll
-      for (int o = 0; o < 2; o++)
+        for (int o = 0; o < 2; o++) load_words<W, true>(to[h][o], &inner[h][g + 8 * o][(s * 4 + c) * 2 * W], 2 * W);
+    };
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-          load_words<W, true>(u[h][o][s], &inner[h][g + 8 * o][(s * 4 + c) * 2 * W], 2 * W);
+    for (int s = 0; s < KS; s++)
+      if (kKeep) load_terms(u[kKeep ? s : 0], s);
     for (uint32_t n0 = n_begin + warp * 32; n0 < n_end; n0 += kWarps * 32) {
       const int at = (int)(n0 + c * 8), valid = (int)n_end - at;
       uint32_t y[2][4];
@@ -402,22 +436,24 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
       const bool here = n0 - n_begin + 32 <= held;  // all of the run's rows of `up` are in shared memory
       float acc[4][4] = {};
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const uint32_t n = n0 + (g >> 1) * 8 + q * 2 + (g & 1);
+      for (int s = 0; s < KS; s++) {
+        const int r = (s * 4 + (int)c) * 2 * W % RP, left = (int)p.rank - r;
+        if (!kKeep) load_terms(u[0], s);
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
+        for (int q = 0; q < 4; q++) {
+          const uint32_t n = n0 + (g >> 1) * 8 + q * 2 + (g & 1);
           uint32_t b[W] = {};
-          const int r = (s * 4 + (int)c) * 2 * W, left = (int)p.rank - r;
           if (here) {
             if (left > 0) load_words<W, VECTOR>(b, up_here + (n - n_begin) * p.rank + r, left);
           } else if (n < n_end && left > 0) {
             load_words<W, VECTOR>(b, up + (size_t)n * p.rank + r, left);
           }
 #pragma unroll
-          for (int h = 0; h < 2; h++)
+          for (int h = 0; h < S::kSlabs; h++)
 #pragma unroll
             for (int w = 0; w < W; w += 2) {
-              const uint32_t a[4] = {u[h][0][s][w], u[h][1][s][w], u[h][0][s][w + 1], u[h][1][s][w + 1]};
+              const auto& x = u[kKeep ? s : 0][h];
+              const uint32_t a[4] = {x[0][w], x[1][w], x[0][w + 1], x[1][w + 1]};
               Half<E>::mma(acc[q], a, b[w], b[w + 1]);
             }
         }
@@ -554,7 +590,7 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
 // prompts: tiles of 128 tokens on the 5th-generation tensor cores
 // ------------------------------------------------------------------------------------
 // Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
-// partial sums in the workspace; the second adds those up, splits them into two 16-bit terms and multiplies
+// partial sums in the workspace; the second adds those up, splits them into three 16-bit terms and multiplies
 // them with `up`, adding `base` on the way out.  In both a tile is so many steps of 64 columns, the tiles of the
 // batch stand one behind the other, and every CTA of a full GPU takes the same number of consecutive
 // steps, so that no number of tiles leaves part of the GPU idle; where a CTA's run starts or ends inside a tile
@@ -696,10 +732,10 @@ template <int RP>
 struct BigShape {
   static constexpr int kDownStage = kRowsBytes + RP * kStep * 2;                // x, down
   static constexpr int kUpStage = kRowsBytes + (RP + 63) / 64 * kStep * 128;    // base, up
-  static constexpr int kTermBytes = (2 * RP + 63) / 64 * kBigTile * 128;        // the rank products: first terms, then second
+  static constexpr int kTermBytes = (kTerms * RP + 63) / 64 * kBigTile * 128;   // the rank products: first terms, then second, then third
   // one CTA an SM, as many stages as fit
   static constexpr int kDownStages = RP <= 32 ? 5 : RP <= 64 ? 4 : 3;
-  static constexpr int kUpStages = RP <= 64 ? 4 : 2;
+  static constexpr int kUpStages = RP <= 32 ? 4 : RP <= 64 ? 3 : 2;
   static constexpr int kDownShared = kDownStages * kDownStage + 1024;
   static constexpr int kUpShared = kUpStages * kUpStage + kTermBytes + 1024;
 };
@@ -958,7 +994,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       const Tile tile = tiles[n];
       const bool bare = tile.group == p.n_groups;
       float back = 1.f;
-      if (!bare) {  // half of the token's rank products a thread: added up, scaled so that the token's largest is in [1, 2), in two terms
+      if (!bare) {  // half of the token's rank products a thread: added up, scaled, in three terms
         constexpr int R = RP / 2;
         const float scale = p.scale ? p.scale[tile.group] : 1.f;
         const uint32_t per = down_share.run(run.tiles);
@@ -978,28 +1014,28 @@ __global__ void __launch_bounds__(kUpThreads, 1)
 #pragma unroll
         for (int c = 0; c < R; c++) {
           u[c] *= scale;
-          top = fmaxf(top, fabsf(u[c]));
+          top = fmaxf(top, size_of(u[c]));
         }
-        top_of[half][row] = top;
-        barrier_arrive(shared_address(&tops));
-        if (!(ok = warp_wait(shared_address(&tops), n & 1))) break;
-        const float s = unit_scale(fmaxf(top, top_of[half ^ 1][row]));
-        back = 1.f / s;
+        float s = 1.f;
+        if (Half<E>::kScaled) {
+          top_of[half][row] = top;
+          barrier_arrive(shared_address(&tops));
+          if (!(ok = warp_wait(shared_address(&tops), n & 1))) break;
+          s = scale_for(fmaxf(top, top_of[half ^ 1][row]));
+          back = 1.f / s;
+        }
 #pragma unroll
         for (int c = 0; c < R; c += 8) {
-          uint32_t hi[4], lo[4];
+          uint32_t term_of[4][kTerms];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float a = u[c + 2 * j] * s, b = u[c + 2 * j + 1] * s;
-            hi[j] = Half<E>::narrow(a, b);
-            const float2 h = Half<E>::widen(hi[j]);
-            lo[j] = Half<E>::narrow(isinf(h.x) ? 0.f : a - h.x, isinf(h.y) ? 0.f : b - h.y);
+          for (int j = 0; j < 4; j++) split<E>(u[c + 2 * j] * s, u[c + 2 * j + 1] * s, term_of[j]);
+#pragma unroll
+          for (int t = 0; t < kTerms; t++) {
+            const uint32_t q = t * (RP / 8) + (half * R + c) / 8, to = term + q / 8 * kBlock64 + piece_at(row, q % 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(term_of[0][t]), "r"(term_of[1][t]),
+                         "r"(term_of[2][t]), "r"(term_of[3][t])
+                         : "memory");
           }
-          const uint32_t q = (half * R + c) / 8, q2 = q + RP / 8;  // the second terms follow the first
-          const uint32_t to = term + q / 8 * kBlock64 + piece_at(row, q % 8);
-          const uint32_t to2 = term + q2 / 8 * kBlock64 + piece_at(row, q2 % 8);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to2), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
         }
       }
       if (!bare) {
@@ -1074,7 +1110,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         order_for_tensor_cores();
         after_sync();
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < kTerms; t++)
 #pragma unroll
           for (int r = 0; r < RP / 16; r++) {
             const int q = t * (RP / 16) + r;  // sixteen ranks of a term
