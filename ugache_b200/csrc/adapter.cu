@@ -1131,12 +1131,14 @@ __global__ void __launch_bounds__(kUpThreads, 1)
 // Tiles of 16 tokens, at most: every group may end in one of its own.
 uint32_t small_tiles(const AdapterParams& p) { return p.n_tokens / kTile + std::min(p.n_groups + 1, p.n_tokens); }
 
+constexpr uint32_t kMostShared = 200 * 1024;  // of a CTA of the kernels below, at most
+
 // A cluster of CTAs a tile.
 template <typename... KArgs, typename... Args>
 cudaError_t cluster_launch(void (*kern)(KArgs...), uint32_t tiles, uint32_t cluster, size_t smem, cudaStream_t stream,
                            const Args&... args) {
-  if (smem > 47 * 1024) {  // beside what is static
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 47 * 1024) {  // beside what is static; the same bound in every call, for another thread may launch the kernel just now
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1169,7 +1171,7 @@ cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t str
   // with four, 16.4 with three).  What is left of it holds `up`.
   constexpr uint32_t kMost = RP <= 32 ? 3 : 2;
   const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, few && RP <= 16 ? 4 : kMost);
-  const uint32_t budget = std::min(216u * 1024 / per_sm, 200u * 1024);
+  const uint32_t budget = std::min(216u * 1024 / per_sm, kMostShared);
   const uint32_t slice = (p.out_dim + cluster * 32 - 1) / (cluster * 32) * 32;
   const uint32_t room = vector ? (uint32_t)std::min<size_t>(budget - S::kShared, (size_t)slice * p.rank * 2) / 16 * 16 : 0;
   return cluster_launch(kern, tiles, cluster, budget, stream, p, room);

@@ -25,11 +25,17 @@ __device__ __forceinline__ uint32_t count_of(const uint32_t* mine, uint32_t rank
   return v;
 }
 
+// Shared memory of a CTA, at most: a plan's, two counts a group and the larger of 32 warps' counts and 8192 ids in order.
+constexpr size_t kMostShared = (kRouteMaxGroups + 1) * 8 + 8192 * 8 + 1024;
+static_assert((kRouteMaxGroups + 1) * 32 * 2 + 8 <= 8192 * 8 + 1024, "the counts are the smaller or fit as well");
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, bool pdl,
                    unsigned cluster, const Args&... args) {
-  if (smem > 36 * 1024) {  // with what is static (up to 9 KB) beyond the 48 KB that need no word
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // with what is static (up to 9 KB) beyond the 48 KB that need no word; the same bound in every call, for another thread
+  // may launch the kernel just now
+  if (smem > 36 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
