@@ -616,19 +616,8 @@ __device__ __forceinline__ Piece piece_within(const char* q, const char* begin, 
   }
   return p;
 }
-// The 16 bytes from `at` (an even address) on, zeros outside the row.
-// `amid`: the row has 16 bytes more on both sides.
-__device__ __forceinline__ Piece piece_anywhere(const char* at, const char* begin, const char* end, bool amid) {
-  const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(at) & 15;
-  const char* q = at - low;
-  Piece a, b;
-  if (amid) {
-    a = *reinterpret_cast<const Piece*>(q);
-    b = *reinterpret_cast<const Piece*>(q + 16);
-  } else {
-    a = piece_within(q, begin, end);
-    b = piece_within(q + 16, begin, end);
-  }
+// The 16 bytes from byte `low` (below 16, even) of a and b on.
+__device__ __forceinline__ Piece shifted(const Piece& a, const Piece& b, uint32_t low) {
   uint32_t w[8] = {a.v[0], a.v[1], a.v[2], a.v[3], b.v[0], b.v[1], b.v[2], b.v[3]};
   if (low & 8) {
 #pragma unroll
@@ -642,6 +631,21 @@ __device__ __forceinline__ Piece piece_anywhere(const char* at, const char* begi
 #pragma unroll
   for (int i = 0; i < 4; i++) p.v[i] = __funnelshift_r(w[i], w[i + 1], (uint32_t)low * 8);  // by low % 4 bytes
   return p;
+}
+// The 16 bytes from `at` (an even address) on, zeros outside the row.
+// `amid`: the row has 16 bytes more on both sides.
+__device__ __forceinline__ Piece piece_anywhere(const char* at, const char* begin, const char* end, bool amid) {
+  const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(at) & 15;
+  const char* q = at - low;
+  Piece a, b;
+  if (amid) {
+    a = *reinterpret_cast<const Piece*>(q);
+    b = *reinterpret_cast<const Piece*>(q + 16);
+  } else {
+    a = piece_within(q, begin, end);
+    b = piece_within(q + 16, begin, end);
+  }
+  return shifted(a, b, low);
 }
 template <typename E>
 __device__ __forceinline__ void store_within(char* q, const Piece& p, char* begin, char* end) {
@@ -677,51 +681,156 @@ __device__ __forceinline__ Floats<E> read_at(const Cut& cut, const char* row, ui
   return x;
 }
 
-// lanes threads a token, as in dots_kernel; `pieces`: cuts of a row, at most.
-template <typename E, bool WEIGHTED, bool DOTS>
-__global__ void __launch_bounds__(kRowsBlock) gather_any_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
+// lanes threads a token, as in dots_kernel; `cuts` of a row, at most.
+template <typename E, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowsBlock) gather_any_kernel(RouteRows p, uint32_t cuts, uint32_t lanes) {
   wait_for_launch_ahead();
   release_launch_behind();
   constexpr int kChoices = 4;
-  __shared__ float share[kRowsBlock / 32][kChoices];
   const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E);
   const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
-  const bool live = t < p.n_tokens;
+  if (t >= p.n_tokens) return;
   const size_t at = (size_t)t * p.k;
-  for (uint32_t j0 = 0; j0 < (DOTS ? p.k : 1); j0 += kChoices) {
-    float dot[kChoices] = {};
-    for (uint32_t u = lane; live && u < pieces; u += lanes) {
-      const uint32_t c = u + 1 < pieces ? u + 1 : 0;  // the row's begin beside its end: one warp has both
-      const Cut cut(row_at(p.token_out, p.token_out_stride, t), bytes, c);
-      if (!cut.inside()) continue;
-      Floats<E> x, sum = {};
-      if (DOTS) x = read_at<E>(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+  for (uint32_t u = lane; u < cuts; u += lanes) {
+    const uint32_t c = u + 1 < cuts ? u + 1 : 0;  // the row's begin beside its end: one warp has both
+    const Cut cut(row_at(p.token_out, p.token_out_stride, t), bytes, c);
+    if (!cut.inside()) continue;
+    Floats<E> sum = {};
 #pragma unroll
-      for (int j = 0; j < kChoices; j++) {
-        const uint32_t row = j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
-        if (row == kNowhere) continue;
-        const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
-        if (WEIGHTED) sum.add(y, p.weights[at + j0 + j]);
-        else sum.add(y);
-        if (DOTS) dot[j] = x.dot(y, dot[j]);
-      }
-      if (j0) continue;
-      for (uint32_t j = kChoices; j < p.k; j++) {  // choices past the first pass join the sum here, their products come later
-        const uint32_t row = place_of(p, at + j);
-        if (row == kNowhere) continue;
-        const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
-        if (WEIGHTED) sum.add(y, p.weights[at + j]);
-        else sum.add(y);
-      }
-      store_within<E>(cut.at, sum.rounded(), cut.begin, cut.end);
+    for (int j = 0; j < kChoices; j++) {
+      const uint32_t row = (uint32_t)j < p.k ? place_of(p, at + j) : kNowhere;
+      if (row == kNowhere) continue;
+      const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
+      if (WEIGHTED) sum.add(y, p.weights[at + j]);
+      else sum.add(y);
     }
-    if (DOTS) share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
+    for (uint32_t j = kChoices; j < p.k; j++) {
+      const uint32_t row = place_of(p, at + j);
+      if (row == kNowhere) continue;
+      const Floats<E> y = read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes);
+      if (WEIGHTED) sum.add(y, p.weights[at + j]);
+      else sum.add(y);
+    }
+    store_within<E>(cut.at, sum.rounded(), cut.begin, cut.end);
+  }
+}
+
+__device__ __forceinline__ void zero_untaken_any(const RouteRows& p, uint32_t bytes, uint32_t cuts) {
+  const uint32_t first = first_untaken(p);
+  const unsigned long long n = (unsigned long long)(p.n_rows - first) * cuts;
+  for (unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x; u < n;
+       u += (unsigned long long)gridDim.x * kRowsBlock) {
+    uint32_t row, c;
+    divide(u, cuts, &row, &c);
+    const Cut cut(row_at(p.row_out, p.row_out_stride, first + row), bytes, c);
+    if (cut.inside()) store_within<uint16_t>(cut.at, Piece{}, cut.begin, cut.end);
   }
 }
 
 // lanes threads a choice: the rows written are cut differently.
-template <typename E, bool WEIGHTED, bool DOTS>
-__global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uint32_t pieces, uint32_t lanes) {
+template <typename E, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uint32_t cuts, uint32_t lanes) {
+  wait_for_launch_ahead();
+  release_launch_behind();
+  const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E);
+  const uint32_t choice = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes, t = choice / p.k;
+  const uint32_t row = choice < p.n_rows ? place_of(p, choice) : kNowhere;
+  const float w = WEIGHTED && row != kNowhere ? p.weights[choice] : 1.f;
+  for (uint32_t u = lane; row != kNowhere && u < cuts; u += lanes) {
+    const uint32_t c = u + 1 < cuts ? u + 1 : 0;
+    const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
+    if (!cut.inside()) continue;
+    const Piece in = piece_of(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
+    Floats<E> x;
+    x.from(in);
+    store_within<E>(cut.at, WEIGHTED ? x.times(w).rounded() : in, cut.begin, cut.end);
+  }
+  zero_untaken_any(p, bytes, cuts);
+}
+
+// Bytes 16 u to 16 u + 15 of a row that starts anywhere, zeros behind it.
+__device__ __forceinline__ Piece piece_of_row(const char* row, uint32_t bytes, uint32_t u) {
+  return piece_anywhere(row + (size_t)u * 16, row, row + bytes, u > 0 && (u + 2) * 16 <= bytes);
+}
+
+// Inner products of rows that start anywhere.  Pieces are counted from the rows' begins, wherever those lie: results do not
+// depend on the addresses, which change with a choice's place.  lanes threads a token (gather) or a choice (spread).
+// 16,384 x 8 rows of 1001 bf16: spread 256 us, the token's row read once more for the cuts (about 330 with pieces exchanged
+// between lanes as in the gather); gathered 198 us (290 with 116 registers a thread).
+struct Share {  // a lane's pieces: its warp has neighbouring ones, `width` of them at a time
+  uint32_t width, seat, begin, end;
+  __device__ __forceinline__ Share(uint32_t lane, uint32_t lanes, uint32_t pieces) {
+    width = min(lanes, 32u);
+    seat = lane & (width - 1);
+    const uint32_t per = (pieces + lanes - 1) / lanes * width;
+    begin = min(lane / width * per, pieces);
+    end = min(begin + per, pieces);
+  }
+};
+
+template <typename E, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowsBlock, sizeof(E) == 4 ? 5 : 4) gather_any_dots_kernel(RouteRows p, uint32_t cuts, uint32_t lanes) {
+  wait_for_launch_ahead();
+  release_launch_behind();
+  constexpr int kChoices = 4;
+  __shared__ float share[kRowsBlock / 32][kChoices];
+  const uint32_t lane = threadIdx.x & (lanes - 1), bytes = p.dim * (uint32_t)sizeof(E), pieces = cuts - 1;
+  const uint32_t t = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes;
+  const bool live = t < p.n_tokens;
+  const size_t at = (size_t)t * p.k;
+  const Share mine(lane, lanes, pieces);
+  for (uint32_t j0 = 0; j0 < p.k; j0 += kChoices) {
+    float dot[kChoices] = {};
+    Piece ahead = {};
+    for (uint32_t u0 = mine.begin; u0 < mine.end; u0 += mine.width) {
+      const uint32_t u = u0 + mine.seat;
+      const bool on = live && u < mine.end;
+      Floats<E> x, sum = {};
+      if (on) x.from(piece_of_row(row_at(p.token_in, p.token_in_stride, t), bytes, u));
+#pragma unroll
+      for (int j = 0; j < kChoices; j++) {
+        const uint32_t row = on && j0 + j < p.k ? place_of(p, at + j0 + j) : kNowhere;
+        if (row == kNowhere) continue;
+        Floats<E> y;
+        y.from(piece_of_row(row_at(p.row_in, p.row_in_stride, row), bytes, u));
+        if (WEIGHTED) sum.add(y, p.weights[at + j0 + j]);
+        else sum.add(y);
+        dot[j] = x.dot(y, dot[j]);
+      }
+      if (j0) continue;
+      for (uint32_t j = kChoices; on && j < p.k; j++) {  // choices past the first pass join the sum here, their products come later
+        const uint32_t row = place_of(p, at + j);
+        if (row == kNowhere) continue;
+        Floats<E> y;
+        y.from(piece_of_row(row_at(p.row_in, p.row_in_stride, row), bytes, u));
+        if (WEIGHTED) sum.add(y, p.weights[at + j]);
+        else sum.add(y);
+      }
+      // What lies between two 16-byte boundaries is the left neighbour's end and the own begin; the first and the last
+      // piece of the warp's run are stored in part.
+      __syncwarp();
+      const Piece out = sum.rounded();
+      const uint32_t neighbour = (threadIdx.x & 31 & ~(mine.width - 1)) | ((mine.seat - 1) & (mine.width - 1));
+      Piece left;
+#pragma unroll
+      for (int i = 0; i < 4; i++) left.v[i] = __shfl_sync(kFull, mine.seat + 1 == mine.width ? ahead.v[i] : out.v[i], neighbour);
+      ahead = out;
+      if (!on) continue;
+      char *row = row_at(p.token_out, p.token_out_stride, t), *q = row + (size_t)u * 16, *end = row + bytes;
+      const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15;
+      if (low == 0) {
+        store_within<E>(q, out, row, end);
+        continue;
+      }
+      store_within<E>(q - low, shifted(left, out, 16 - low), u == mine.begin ? q : row, end);
+      if (u + 1 == mine.end) store_within<E>(q - low + 16, shifted(out, out, 16 - low), row, q + 16 < end ? q + 16 : end);
+    }
+    share_sums<kChoices>(dot, share, p, at, j0, live, lane, lanes);
+  }
+}
+
+template <typename E, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowsBlock, 6) spread_any_dots_kernel(RouteRows p, uint32_t cuts, uint32_t lanes) {
   wait_for_launch_ahead();
   release_launch_behind();
   __shared__ float share[kRowsBlock / 32][1];
@@ -729,27 +838,25 @@ __global__ void __launch_bounds__(kRowsBlock) spread_any_kernel(RouteRows p, uin
   const uint32_t choice = blockIdx.x * (kRowsBlock / lanes) + threadIdx.x / lanes, t = choice / p.k;
   const uint32_t row = choice < p.n_rows ? place_of(p, choice) : kNowhere;
   const float w = WEIGHTED && row != kNowhere ? p.weights[choice] : 1.f;
+  const char *from = row_at(p.token_in, p.token_in_stride, t), *other = row_at(p.row_in, p.row_in_stride, row);
   float dot[1] = {};
-  for (uint32_t u = lane; row != kNowhere && u < pieces; u += lanes) {
-    const uint32_t c = u + 1 < pieces ? u + 1 : 0;
-    const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, c);
+  const Share mine(lane, lanes, cuts - 1);
+  const uint32_t end = mine.begin < mine.end && mine.end + 1 == cuts ? cuts : mine.end;  // one cut more than pieces
+  for (uint32_t u = mine.begin + mine.seat; row != kNowhere && u < end; u += mine.width) {
+    Floats<E> x, y;
+    if (u + 1 < cuts) {
+      x.from(piece_of_row(from, bytes, u));
+      y.from(piece_of_row(other, bytes, u));
+      dot[0] = x.dot(y, dot[0]);
+    }
+    const Cut cut(row_at(p.row_out, p.row_out_stride, row), bytes, u + 1 < cuts ? u + 1 : 0);
     if (!cut.inside()) continue;
-    const Piece in = piece_of(cut, row_at(p.token_in, p.token_in_stride, t), bytes);
-    Floats<E> x;
+    const Piece in = piece_of(cut, from, bytes);  // again, from the L1
     x.from(in);
-    if (DOTS) dot[0] = x.dot(read_at<E>(cut, row_at(p.row_in, p.row_in_stride, row), bytes), dot[0]);
     store_within<E>(cut.at, WEIGHTED ? x.times(w).rounded() : in, cut.begin, cut.end);
   }
-  if (DOTS) share_sums<1>(dot, share, p, choice, 0, choice < p.n_rows, lane, lanes);
-  const uint32_t first = first_untaken(p);
-  const unsigned long long n = (unsigned long long)(p.n_rows - first) * pieces;
-  for (unsigned long long u = (unsigned long long)blockIdx.x * kRowsBlock + threadIdx.x; u < n;
-       u += (unsigned long long)gridDim.x * kRowsBlock) {
-    uint32_t row, c;
-    divide(u, pieces, &row, &c);
-    const Cut cut(row_at(p.row_out, p.row_out_stride, first + row), bytes, c);
-    if (cut.inside()) store_within<E>(cut.at, Piece{}, cut.begin, cut.end);
-  }
+  share_sums<1>(dot, share, p, choice, 0, choice < p.n_rows, lane, lanes);
+  zero_untaken_any(p, bytes, cuts);
 }
 
 // Whether every row in use starts on a 16-byte boundary and is whole pieces long.
@@ -784,8 +891,10 @@ cudaError_t rows_launch(const RouteRows& p, bool spread, cudaStream_t stream) {
   auto per_token = [&](auto kern, uint32_t pieces, uint32_t each) { return per_row(kern, p.n_tokens, pieces, each); };
   if (!rows_aligned(p, sizeof(E))) {
     const uint32_t cuts = (uint32_t)((bytes + 15) / 16 + 1);
-    if (spread) return per_row(p.dots ? spread_any_kernel<E, WEIGHTED, true> : spread_any_kernel<E, WEIGHTED, false>, p.n_rows, cuts, p.dots ? 2 : 4);
-    return per_token(p.dots ? gather_any_kernel<E, WEIGHTED, true> : gather_any_kernel<E, WEIGHTED, false>, cuts, p.dots ? 2 : 1);
+    if (p.dots && spread) return per_row(spread_any_dots_kernel<E, WEIGHTED>, p.n_rows, cuts, 4);
+    if (p.dots) return per_token(gather_any_dots_kernel<E, WEIGHTED>, cuts, 4);
+    if (spread) return per_row(spread_any_kernel<E, WEIGHTED>, p.n_rows, cuts, 4);
+    return per_token(gather_any_kernel<E, WEIGHTED>, cuts, 1);
   }
   const uint32_t pieces = (uint32_t)(bytes / 16);
   if (p.dots) {
