@@ -490,9 +490,9 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
                     const float* scale, const int32_t* offsets, const int32_t* order, size_t n_tokens,
                     int n_groups, size_t rank, size_t dim, size_t out_dim, void* out, int64_t out_stride,
                     void* workspace, size_t workspace_bytes, void* stream);
-/* The prompt kernels wait for their own copies and products; a wait that does not end within about two
- * seconds ends the kernel (its outputs are then unfinished) and is counted per GPU.  Reads that count,
- * synchronising; 0 on a sound machine. */
+/* The kernels of 16-bit adapters wait for their own copies and products; a wait that does not end within about
+ * two seconds ends the kernel (what it has not stored by then stays as it was) and is counted per GPU.  The call has
+ * returned long since: who wants to know reads this count, which synchronises; 0 on a sound machine. */
 int ugc_adapter_stalled(int device_id, uint32_t* count);
 
 /* -- introspection --------------------------------------------------------------------- */

@@ -179,6 +179,8 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     }
   }
 }
+// By a whole warp, which stays together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(kFull, barrier_wait(bar, parity)); }
 
 // ------------------------------------------------------------------------------------
 // single tokens: a cluster of CTAs has a tile of 16 tokens
@@ -262,7 +264,8 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   if (tile.count == 0) return;  // of the whole cluster
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const uint32_t n_slice = (p.out_dim + members * 32 - 1) / (members * 32) * 32;
-  const uint32_t n_begin = min(p.out_dim, member * n_slice), n_end = min(p.out_dim, n_begin + n_slice);
+  const uint32_t n_begin = min(p.out_dim, member * n_slice);
+  uint32_t n_end = min(p.out_dim, n_begin + n_slice);
   const uint16_t* up = static_cast<const uint16_t*>(p.up) + (long long)tile.group * p.up_stride;
   const bool bare = tile.group == p.n_groups;
   const uint32_t held = VECTOR && !bare ? min(n_end - n_begin, up_room / 2 / p.rank) : 0;  // rows of `up` to bring here
@@ -403,7 +406,10 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
   }
   __syncthreads();
   cluster_arrive();  // waited for at the end: nobody leaves while its sums are being read
-  if (held) barrier_wait(shared_address(&up_landed), 0);
+  if (held && !warp_wait(shared_address(&up_landed), 0)) {
+    warp_wait(shared_address(&up_landed), 0);  // once more: the copy's target is the CTA's own memory
+    n_end = n_begin;                           // nothing is stored
+  }
   __syncwarp();
 
   // second product: every CTA a slice of out_dim, 32 of it a warp at a time.  Column 2c + b of the
@@ -615,8 +621,6 @@ constexpr int kDownThreads = kProducers + 128 + 32;         // copy, take out, m
 constexpr int kUpThreads = kProducers + 256 + 32;
 constexpr int kMostTiles = 36;                              // a CTA's run touches
 
-// By a whole warp, which stays together.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(kFull, barrier_wait(bar, parity)); }
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }

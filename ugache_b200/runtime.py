@@ -402,6 +402,16 @@ def adapter_add(base, x, down, up, plan, scale=None, out=None, stream=None):
     return (_lib._fast or _lib.fast()).adapter_add(base, x, down, up, plan.offsets, plan.order, scale, out, stream)
 
 
+def adapter_stalled(device=0):
+    """Waits inside the adapter kernels of this GPU that ran out (after about two seconds, of a copy or a product of the
+    kernel's own) since the library was loaded: 0 on a sound machine.  Otherwise outputs of ``adapter_add`` are
+    unfinished, which the calls themselves, long returned by then, cannot say.  Synchronises: for a health check,
+    not for every step."""
+    n = C.c_uint32(0)
+    check(_lib.lib().ugc_adapter_stalled(int(device), C.byref(n)))
+    return int(n.value)
+
+
 def gen_table(dst_ptr, seed, row_begin, n_rows, dim, elem_bytes, stream=0):
     check(_lib.lib().ugc_gen_table(C.c_void_p(dst_ptr), seed, row_begin, n_rows, dim, elem_bytes,
                                    C.c_void_p(stream)))
