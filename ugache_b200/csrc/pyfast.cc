@@ -269,6 +269,13 @@ bool unpack(PyObject* o, const char* name, at::Tensor* t) {
   return true;
 }
 
+// The caller's own tensor has been written: what autograd saved of it before is no longer there.
+void written(PyObject* o) {
+  if (o == Py_None) return;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The call's stream, from its stream argument and the device of its first tensor.  A stream that is named
 // becomes the current one meanwhile: what the call allocates or copies belongs to it.
 struct OnStream {
@@ -427,6 +434,7 @@ PyObject* fast_route_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
                             (size_t)x.size(1), op, row_stride(out), on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
+  written(a[4]);
   return THPVariable_Wrap(std::move(out));
   UGC_PY_END
 }
@@ -457,6 +465,7 @@ PyObject* fast_route_dispatch_grad(PyObject*, PyObject* const* a, Py_ssize_t n_a
                                  (size_t)p.tokens, (size_t)p.k, (size_t)dout.size(1), op, row_stride(dx), dp, on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
+  written(a[5]);
   return pair(std::move(dx), std::move(dw));
   UGC_PY_END
 }
@@ -484,6 +493,7 @@ PyObject* fast_route_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                            (size_t)rows.size(1), op, row_stride(out), on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
+  written(a[4]);
   return THPVariable_Wrap(std::move(out));
   UGC_PY_END
 }
@@ -514,6 +524,7 @@ PyObject* fast_route_combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_ar
                                 (size_t)p.tokens, (size_t)p.k, (size_t)dy.size(1), op, row_stride(drows), dp, on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
+  written(a[5]);
   return pair(std::move(drows), std::move(dw));
   UGC_PY_END
 }
@@ -569,6 +580,7 @@ PyObject* fast_adapter_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                          op, row_stride(out), wp, bytes, on.stream);
   Py_END_ALLOW_THREADS
   if (rc != UGC_OK) return raise_status(rc);
+  written(a[7]);
   return THPVariable_Wrap(std::move(out));
   UGC_PY_END
 }

@@ -350,6 +350,7 @@ class Cache:
 
 
 # -- routing: tokens grouped by the expert or adapter that serves them --------------------------
+# An output that the caller gives counts as changed in place for autograd.
 class RoutePlan(NamedTuple):
     """A batch of ids sorted by group, as ``route_plan`` makes it (all int32, on the GPU).
 
