@@ -6,6 +6,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -269,6 +270,12 @@ bool unpack(PyObject* o, const char* name, at::Tensor* t) {
   return true;
 }
 
+// The calls record nothing for autograd: a gradient that somebody waits for would be missing without a word.
+bool not_recorded(const at::Tensor& t, const char* name) {
+  if (!t.requires_grad() || !at::GradMode::is_enabled()) return true;
+  return bad(PyExc_ValueError, "%s requires a gradient, which this call does not record: use it inside a torch.autograd.Function or under torch.no_grad()", name);
+}
+
 // The caller's own tensor has been written: what autograd saved of it before is no longer there.
 void written(PyObject* o) {
   if (o == Py_None) return;
@@ -295,7 +302,7 @@ struct OnStream {
 bool rows_arg(PyObject* o, const char* name, Call* c, int64_t n, bool more, int64_t dim, bool output, at::Tensor* t) {
   if (!unpack(o, name, t)) return false;
   if (t->dim() != 2) return bad(PyExc_ValueError, "%s must have two dimensions", name);
-  if (!on_device(c, *t, name)) return false;
+  if (!on_device(c, *t, name) || !not_recorded(*t, name)) return false;
   const at::ScalarType ty = t->scalar_type();
   if (ty != at::kFloat && ty != at::kHalf && ty != at::kBFloat16)
     return bad(PyExc_TypeError, "%s must be float32, float16 or bfloat16", name);
@@ -329,7 +336,7 @@ int elem_type(const Call& c) {
 
 // A plan's array of int32, or fp32 values per choice; dense, so a copy is made of anything else.
 bool words_arg(PyObject* o, const char* name, Call* c, at::ScalarType ty, int64_t numel, at::Tensor* t) {
-  if (!unpack(o, name, t) || !on_device(c, *t, name)) return false;
+  if (!unpack(o, name, t) || !on_device(c, *t, name) || !not_recorded(*t, name)) return false;
   if (t->scalar_type() != ty) return bad(PyExc_TypeError, ty == at::kInt ? "%s must be int32" : "%s must be float32", name);
   if (numel >= 0 && t->numel() != numel) {
     PyErr_Format(PyExc_ValueError, "%s has %lld elements, %lld expected", name, (long long)t->numel(), (long long)numel);
@@ -533,7 +540,7 @@ PyObject* fast_route_combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_ar
 bool adapters_arg(PyObject* o, const char* name, Call* c, at::Tensor* t) {
   if (!unpack(o, name, t)) return false;
   if (t->dim() != 3) return bad(PyExc_ValueError, "%s must have three dimensions", name);
-  if (!on_device(c, *t, name)) return false;
+  if (!on_device(c, *t, name) || !not_recorded(*t, name)) return false;
   if (t->scalar_type() != c->ty) return bad(PyExc_TypeError, "%s has another type than base", name);
   const int64_t d = t->size(2);
   if ((d > 1 && t->stride(2) != 1) || (t->size(1) > 1 && t->stride(1) != d) ||

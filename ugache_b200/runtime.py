@@ -350,7 +350,9 @@ class Cache:
 
 
 # -- routing: tokens grouped by the expert or adapter that serves them --------------------------
-# An output that the caller gives counts as changed in place for autograd.
+# The calls record nothing for autograd: rows, weights or adapters that require a gradient are refused with a ValueError
+# unless gradients are off, as they are under torch.no_grad() and inside a torch.autograd.Function, where these are the
+# forward and the backward.  An output that the caller gives counts as changed in place.
 class RoutePlan(NamedTuple):
     """A batch of ids sorted by group, as ``route_plan`` makes it (all int32, on the GPU).
 
