@@ -72,3 +72,27 @@ def test_ranks_of_far_magnitudes(rt, rank, T, elem):
     want = inner @ up[0].double().t()
     off = (2.0 ** -23 * inner + 2.0 ** -38 * 2) @ up[0].double().t()
     assert bool(((got.double() - want).abs() <= off + torch.finfo(ty).eps / 2 * (want + off)).all())
+
+
+@pytest.mark.parametrize("elem", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rank", [1, 4, 8, 12, 16, 24, 40, 72, 128])
+@pytest.mark.parametrize("T", [50, 6000])
+def test_an_infinite_input_is_an_infinite_result(rt, rank, T, elem):
+    """All factors of a token's infinite element are positive, and so is every product that `up` makes of an output's
+    sign: the formula has infinities of one sign in each output, and no NaN, whatever the rank is padded to."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rank)
+    ty = torch.float32 if elem == "f32" else TYPES[elem]
+    x, base = torch.rand((T, 64), generator=g, device="cuda"), torch.randn((T, 72), generator=g, device="cuda")
+    down, up = 0.5 + torch.rand((2, rank, 64), generator=g, device="cuda"), 0.5 + torch.rand((2, 72, rank), generator=g, device="cuda")
+    up[:, 1::2] *= -1
+    x[3, 10], x[T - 1, 63] = float("inf"), float("-inf")
+    ids = torch.randint(0, 2, (T,), generator=g, device="cuda")
+    got = run(rt, base.to(ty), x.to(ty), down.to(ty), up.to(ty), ids)
+    sign = torch.ones(72, device="cuda")
+    sign[1::2] = -1
+    inf = float("inf")
+    assert torch.equal(got[3].float(), inf * sign) and torch.equal(got[T - 1].float(), -inf * sign)
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[3], rest[T - 1] = False, False
+    assert bool(torch.isfinite(got[rest]).all())

@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 #pragma unroll
           for (int w = 0; w < kMostCluster; w++)
             if (w < members) u[o].x += v[w].x, u[o].y += v[w].y;
-          u[o].x *= scale, u[o].y *= scale;
+          // beyond the rank are no products: an infinite x would leave NaN there
+          u[o] = make_float2(r < p.rank ? u[o].x * scale : 0.f, r + 1 < p.rank ? u[o].y * scale : 0.f);
         }
         top = fmaxf(top, fmaxf(size_of(u[o].x), size_of(u[o].y)));
       }
@@ -1017,7 +1018,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         }
 #pragma unroll
         for (int c = 0; c < R; c++) {
-          u[c] *= scale;
+          u[c] = half * R + c < p.rank ? u[c] * scale : 0.f;  // an infinite x leaves NaN beyond the rank
           top = fmaxf(top, size_of(u[c]));
         }
         float s = 1.f;
