@@ -96,3 +96,19 @@ def test_an_infinite_input_is_an_infinite_result(rt, rank, T, elem):
     rest = torch.ones(T, dtype=torch.bool, device="cuda")
     rest[3], rest[T - 1] = False, False
     assert bool(torch.isfinite(got[rest]).all())
+
+
+@pytest.mark.parametrize("elem", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("T,rank", [(50, 16), (50, 3), (6000, 16)])
+def test_tokens_without_an_adapter_keep_their_bits(rt, T, rank, elem):
+    """Negative zeros, subnormals and infinities among them."""
+    ty = torch.float32 if elem == "f32" else TYPES[elem]
+    base = torch.randn(T, 88, device="cuda").to(ty)
+    base[:, ::4], base[:, 1::8] = -0.0, float("-inf")
+    base[:, 2::8] = torch.finfo(ty).smallest_normal / 4
+    ids = torch.randint(0, 3, (T,), device="cuda")
+    ids[::2] = -1
+    x, down, up = torch.randn(T, 48, device="cuda").to(ty), torch.randn(3, rank, 48, device="cuda").to(ty), torch.randn(3, 88, rank, device="cuda").to(ty)
+    got = run(rt, base, x, down, up, ids)
+    bits = torch.int32 if elem == "f32" else torch.int16
+    assert torch.equal(got[::2].view(bits), base[::2].view(bits))

@@ -561,11 +561,18 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
     cluster_arrive();  // waited for at the end: nobody leaves while its sums are being read
   }
   const uint32_t n_slice = (p.out_dim + members - 1) / members, n_end = min(p.out_dim, (member + 1) * n_slice);
-  const float* up = static_cast<const float*>(p.up) + (bare ? 0 : (long long)tile.group * p.up_stride);
+  if (bare) {  // bit for bit: a sum with 0 would turn -0 into 0
+    for (uint32_t n = member * n_slice + threadIdx.x; n < n_end; n += kBlock)
+#pragma unroll
+      for (int m = 0; m < kTile; m++)
+        if (token[m] >= 0) out[(long long)token[m] * p.out_stride + n] = base[(long long)token[m] * p.base_stride + n];
+    return;
+  }
+  const float* up = static_cast<const float*>(p.up) + (long long)tile.group * p.up_stride;
   const bool vector = rank % 4 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0;
   for (uint32_t n = member * n_slice + threadIdx.x; n < n_end; n += kBlock) {
     float acc[kTile] = {};
-    for (uint32_t r = 0; !bare && r < rank; r += 4) {
+    for (uint32_t r = 0; r < rank; r += 4) {
       float u[4] = {};
       if (vector) {
         const float4 v = *reinterpret_cast<const float4*>(up + (size_t)n * rank + r);
@@ -590,7 +597,7 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
     for (int m = 0; m < kTile; m++)
       if (token[m] >= 0) out[(long long)token[m] * p.out_stride + n] = base[(long long)token[m] * p.base_stride + n] + acc[m];
   }
-  if (!bare) cluster_wait();
+  cluster_wait();
 }
 
 // ------------------------------------------------------------------------------------
