@@ -1,7 +1,8 @@
 """Plan, dispatch and combine where sizes and addresses decide what is read and added when."""
+import numpy as np
 import pytest
 
-from tests.test_gpu_routing import Case
+from tests.test_gpu_routing import Case, check_plan
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -40,3 +41,33 @@ def test_products_of_odd_rows_do_not_depend_on_the_batch(rt, elem, dim, k):
         two = rt.route_combine_grad(x, plan, weights=w, rows=rows)
         assert torch.equal(one[0], dx[part]) and torch.equal(one[1], dw[part])
         assert torch.equal(two[0][at], drows[whole]) and torch.equal(two[1], dw[part])
+
+
+# one CTA up to 1024 ids, a cluster of eight up to 65,536 (its tiles full there), parts beyond
+@pytest.mark.parametrize("n", [65528, 65535, 65536, 151552, 151553])
+@pytest.mark.parametrize("G", [1, 256, 1024])
+def test_plans_at_the_largest_cluster(rt, n, G):
+    check_plan(rt, np.random.default_rng(n + G).integers(-1, G + 1, n), G)
+
+
+# From 148 * 2048 * 4 pieces of 16 bytes on a thread has several: four with up to two choices and where pieces come in
+# fours, else two, else one.
+@pytest.mark.parametrize("elem,dim", [("bf16", 2048), ("f16", 2064), ("bf16", 2056), ("f32", 1024), ("f32", 1032), ("f32", 1028)])
+@pytest.mark.parametrize("k", [1, 2, 3, 5])
+@pytest.mark.parametrize("weighted", [True, False])
+def test_rows_of_large_batches(rt, elem, dim, k, weighted):
+    T = 4900
+    c = Case(rt, T, k, dim, elem, G=5, dropped=0.1, weighted=weighted)
+    assert T * (dim * c.ty.itemsize // 16) >= 148 * 2048 * 4
+    y = rt.route_combine(c.rows, c.plan, weights=c.w)
+    dx, none = rt.route_dispatch_grad(c.rows, c.plan, weights=c.w)
+    assert none is None and torch.equal(dx, y)
+    c.check_gathered(y)
+    # the same tokens in a small batch: bit for bit
+    ids = torch.full((T, k), -1, dtype=torch.int64, device="cuda")
+    ids[c.taken] = torch.bucketize(c.pos[c.taken], c.plan.offsets.long()[1:], right=True)
+    for part in (slice(0, 9), slice(T - 20, T)):
+        plan = rt.route_plan(ids[part].contiguous(), 5)
+        rows = torch.zeros((ids[part].numel(), dim), dtype=c.ty, device="cuda")
+        rows[plan.position[plan.position >= 0].long()] = c.rows[c.pos[part][c.taken[part]]]
+        assert torch.equal(rt.route_combine(rows, plan, weights=None if c.w is None else c.w[part].contiguous()), y[part])
