@@ -112,3 +112,26 @@ def test_tokens_without_an_adapter_keep_their_bits(rt, T, rank, elem):
     got = run(rt, base, x, down, up, ids)
     bits = torch.int32 if elem == "f32" else torch.int16
     assert torch.equal(got[::2].view(bits), base[::2].view(bits))
+
+
+@pytest.mark.parametrize("rank", [16, 64, 128])
+@pytest.mark.parametrize("T", [50, 6000])
+def test_long_sums_of_one_sign(rt, T, rank):
+    """Every factor is positive, so that whatever a sum cuts off adds up; `up` hands the rank products out one by one and
+    `base` takes away what the result's type could hide.  Bound, of the sum: 2^-23 for each instruction of a matrix unit's
+    own sum (prompts: 8; single tokens: 4, at rank 16 the 32 that a warp has of a row), 2^-24 for each fp32 addition behind it
+    (prompts: 128 steps and at most 8 parts; single tokens: the sums of a warp, and those of 16 warps and 8 CTAs at most),
+    2^-23 for each of the three terms and for the scale."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T + rank)
+    G, dim = 2, 16384
+    x, down = torch.rand((T, dim), generator=g, device="cuda").half(), (torch.rand((G, rank, dim), generator=g, device="cuda") / 64).half()
+    up = torch.eye(rank, device="cuda").expand(G, rank, rank).contiguous().half()
+    ids = torch.randint(0, G, (T,), generator=g, device="cuda")
+    delta = torch.stack([x.double() @ down[a].double().t() for a in range(G)])[ids, torch.arange(T, device="cuda")]
+    base = (-delta).half()
+    got = run(rt, base, x, down, up, ids)
+    want = base.double() + delta
+    own, added = (8, 136) if T > 1000 else (32, 24) if rank == 16 else (4, {64: 16, 128: 32}[rank] + 24)
+    off = (own * 2.0 ** -23 + added * 2.0 ** -24 + 4 * 2.0 ** -23) * delta
+    assert bool(((got.double() - want).abs() <= off + torch.finfo(torch.float16).eps / 2 * (want.abs() + off) + 2.0 ** -25).all())

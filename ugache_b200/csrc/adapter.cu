@@ -323,13 +323,21 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
         }
       }
 #pragma unroll
-      for (int f = 0; f < kFlight; f++) {
-        const uint32_t a0[4] = {r0[f][0], r1[f][0], r0[f][1], r1[f][1]}, a1[4] = {r0[f][2], r1[f][2], r0[f][3], r1[f][3]};
+      for (int r = 0; r < RT; r++) {
+        // The matrix unit cuts its sums off, always towards zero, which adds up: where few warps share a row, four
+        // instructions are a sum of their own (16,384 columns of one sign, rank 128: 2e-7 off instead of 6e-6).  Up to rank 32
+        // a warp has at most 1/32 of the row, and no register to spare.
+        float own[4] = {};
+        float (&sum)[4] = RP >= 64 ? own : acc[r];
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-          Half<E>::mma(acc[r], a0, b[f][r][0], b[f][r][1]);
-          Half<E>::mma(acc[r], a1, b[f][r][2], b[f][r][3]);
+        for (int f = 0; f < kFlight; f++) {
+          const uint32_t a0[4] = {r0[f][0], r1[f][0], r0[f][1], r1[f][1]}, a1[4] = {r0[f][2], r1[f][2], r0[f][3], r1[f][3]};
+          Half<E>::mma(sum, a0, b[f][r][0], b[f][r][1]);
+          Half<E>::mma(sum, a1, b[f][r][2], b[f][r][3]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (RP >= 64) acc[r][i] += own[i];
       }
     }
     float* mine = part + (size_t)depth_group * kTile * RP + rank0;
@@ -456,7 +464,7 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
             load_words<W, VECTOR>(b, up + (size_t)n * p.rank + r, left);
           }
 #pragma unroll
-          for (int h = 0; h < S::kSlabs; h++)
+          for (int h = S::kSlabs - 1; h >= 0; h--)  // the small terms first
 #pragma unroll
             for (int w = 0; w < W; w += 2) {
               const auto& x = u[kKeep ? s : 0][h];
@@ -835,7 +843,7 @@ __device__ Run find_run(const AdapterParams& p, const BigShare& share, bool bare
 template <typename E, int RP>
 __global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterParams p, float* __restrict__ inner, BigShare share) {
   using S = BigShape<RP>;
-  constexpr int kStages = S::kDownStages, kColumns = 2 * RP;
+  constexpr int kStages = S::kDownStages, kColumns = 2 * RP, kLoads = RP < 64 ? RP / 16 : 4;
   extern __shared__ unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], ready[2], taken[2];
   __shared__ uint32_t tmem_slot;
@@ -881,53 +889,61 @@ __global__ void __launch_bounds__(kDownThreads, 1) adapter_down_kernel(AdapterPa
     }
     copies_done();
   } else if (warp < 8) {
+    // The matrix unit cuts its sums off at 24 bits, always towards zero: over the 256 instructions of 4096 columns of one
+    // sign that made 7e-6 of the sum.  So a step's products (8 instructions) are a sum of their own, added up here.
     const uint32_t row = threadIdx.x - kProducers;
-    for (uint32_t n = 0; n < run.count; n++) {
+    uint32_t i = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok && n < run.count; n++) {
       const Tile tile = tiles[n];
-      if (!warp_wait(shared_address(&ready[n & 1]), n / 2 & 1)) break;
-      after_sync();
+      float sum[RP / 16][16];
+#pragma unroll
+      for (int c = 0; c < RP; c++) sum[c / 16][c % 16] = 0.f;
+      for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
+        if (!(ok = warp_wait(shared_address(&ready[i & 1]), i / 2 & 1))) break;
+        after_sync();
+#pragma unroll
+        for (int c0 = 0; c0 < RP / 16; c0 += kLoads) {
+          float v[kLoads][16];
+#pragma unroll
+          for (int c = 0; c < kLoads; c++) from_tensor_memory(v[c], tmem + ((warp - 4) * 32 << 16) + (i & 1) * RP + (c0 + c) * 16);
+          loads_done(v);
+#pragma unroll
+          for (int c = 0; c < kLoads * 16; c++) sum[c0 + c / 16][c % 16] += v[c / 16][c % 16];
+        }
+        before_sync();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_address(&taken[i & 1]));
+      }
+      if (!ok) break;
       const uint32_t part = blockIdx.x - (uint32_t)((unsigned long long)(run.first + n) * run.tile_steps / share.run(run.tiles));
       float* to = inner + ((size_t)part * p.n_tokens + tile.first) * RP + row * 4;
+      if (row < tile.count) {
 #pragma unroll
-      for (int c0 = 0; c0 < RP; c0 += 64) {
-        constexpr int kLoads = RP < 64 ? RP / 16 : 4;
-        float v[kLoads][16];
-#pragma unroll
-        for (int c = 0; c < kLoads; c++) from_tensor_memory(v[c], tmem + ((warp - 4) * 32 << 16) + (n & 1) * RP + c0 + c * 16);
-        loads_done(v);
-        if (row < tile.count) {
-#pragma unroll
-          for (int c = 0; c < kLoads; c++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(to + (size_t)(c0 + c * 16 + i) * tile.count) = make_float4(v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3]);
+        for (int c = 0; c < RP; c += 4) {
+          const float* s = &sum[c / 16][c % 16];
+          *reinterpret_cast<float4*>(to + (size_t)c * tile.count) = make_float4(s[0], s[1], s[2], s[3]);
         }
       }
-      before_sync();
-      __syncwarp();
-      if (lane == 0) barrier_arrive(shared_address(&taken[n & 1]));
     }
   } else if (lane == 0) {
     uint32_t i = 0;
     bool ok = true;
-    for (uint32_t n = 0; ok && n < run.count; n++) {
-      if (n >= 2 && !barrier_wait(shared_address(&taken[n & 1]), (n / 2 - 1) & 1)) break;
-      bool add = false;
+    for (uint32_t n = 0; ok && n < run.count; n++)
       for (uint32_t k = run.from(n), end = run.to(n); k < end; k++, i++) {
         const uint32_t s = i % kStages, at = ring + s * S::kDownStage;
-        if (!(ok = barrier_wait(shared_address(&full[s]), i / kStages & 1))) break;
+        ok = barrier_wait(shared_address(&full[s]), i / kStages & 1) &&
+             (i < 2 || barrier_wait(shared_address(&taken[i & 1]), (i / 2 - 1) & 1));
+        if (!ok) break;
         order_for_tensor_cores();
         after_sync();
 #pragma unroll
-        for (int q = 0; q < kStep / 16; q++) {
-          multiply(tmem + (n & 1) * RP, operand(at + q / 4 * kBlock64 + q % 4 * 32),
-                   operand(at + kRowsBytes + q / 4 * (RP * 128) + q % 4 * 32), instruction<E>(RP), add);
-          add = true;
-        }
+        for (int q = 0; q < kStep / 16; q++)
+          multiply(tmem + (i & 1) * RP, operand(at + q / 4 * kBlock64 + q % 4 * 32),
+                   operand(at + kRowsBytes + q / 4 * (RP * 128) + q % 4 * 32), instruction<E>(RP), q > 0);
         arrive_behind_products(shared_address(&empty[s]));
+        arrive_behind_products(shared_address(&ready[i & 1]));
       }
-      if (ok) arrive_behind_products(shared_address(&ready[n & 1]));
-    }
   }
   before_sync();
   __syncthreads();
@@ -1122,13 +1138,11 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         order_for_tensor_cores();
         after_sync();
 #pragma unroll
-        for (int t = 0; t < kTerms; t++)
-#pragma unroll
-          for (int r = 0; r < RP / 16; r++) {
-            const int q = t * (RP / 16) + r;  // sixteen ranks of a term
-            multiply(tmem + (i & 1) * kStep, operand(term + q / 4 * kBlock64 + q % 4 * 32),
-                     operand(at + r / 4 * (kStep * 128) + r % 4 * 32), instruction<E>(kStep), q > 0);
-          }
+        for (int q = kTerms * (RP / 16) - 1; q >= 0; q--) {  // sixteen ranks of a term; the small terms first, while little is cut off
+          const int r = q % (RP / 16);
+          multiply(tmem + (i & 1) * kStep, operand(term + q / 4 * kBlock64 + q % 4 * 32),
+                   operand(at + r / 4 * (kStep * 128) + r % 4 * 32), instruction<E>(kStep), q < kTerms * (RP / 16) - 1);
+        }
         arrive_behind_products(shared_address(&product[i & 1]));
       }
     }
