@@ -452,11 +452,12 @@ int ugc_route_plan(int device_id, const void* ids, int id_bytes, size_t n_tokens
  *                  dweights[t,j] = <dy[t], rows[position[t,j]]>      (only if dweights is given)
  *
  * Sums and products are fp32, the choices of a token added in their order by fused multiply-adds,
- * one rounding at the end; the order of the additions of dweights is fixed by dim, k and whether all rows
- * start on 16-byte boundaries, never by the number of tokens.  A choice whose position is -1 (or
- * outside the rows) adds nothing, its row is not read and its dweights are 0; a token without any
- * choice gets zeros.  Rows of `out` and `drows` from `routed` on, which no choice takes, are zeroed;
- * routed NULL: left as they were.  x / rows may be NULL in the gradients if dweights is. */
+ * one rounding at the end; the order of the additions of dweights is fixed by dim, k and whether all
+ * rows start on 16-byte boundaries, never by the number of tokens or a row's place.  A choice whose
+ * position is -1 (or outside the rows) adds nothing, its row is not read and its dweights are 0; a
+ * token without any choice gets zeros.  Rows of `out` and `drows` from `routed` on, which no choice
+ * takes, are zeroed; routed NULL: left as they were.  x / rows may be NULL in the gradients if
+ * dweights is. */
 int ugc_route_dispatch(int device_id, int elem_type, const void* x, int64_t x_stride, const float* weights,
                        const int32_t* position, const int32_t* routed, size_t n_tokens, size_t k, size_t dim,
                        void* out, int64_t out_stride, void* stream);
@@ -478,11 +479,15 @@ int ugc_route_combine_grad(int device_id, int elem_type, const void* dy, int64_t
  * elements apart -- so a row of an adapter table looked up through the cache can hold both, and the
  * `inverse` of ugc_lookup_unique is the plan's ids.  scale: fp32 per adapter, or NULL for 1.
  * out may be base itself (same stride); other overlaps are not allowed.  Rank at most
- * UGC_ADAPTER_MAX_RANK.  fp16 and bf16 run on the matrix units (fp32 does not, and is many times slower): 16-byte aligned addresses and strides, dims and ranks in multiples of 8
- * elements take the fast loads.  Sums are fp32; the rank products enter the second product as three
- * 16-bit terms, which hold all 24 bits of the sum (fp16: of those down to 2^-16 of the token's largest,
- * below that 2^-39 of the largest); infinities in an adapter that a token uses may come out as NaN.  workspace: ugc_adapter_workspace bytes (0 for small
- * batches, then NULL will do), 16-byte aligned, free again when the call's work is done. */
+ * UGC_ADAPTER_MAX_RANK.  fp16 and bf16 run on the matrix units (fp32 does not, and is many times
+ * slower): 16-byte aligned addresses and strides, dims and ranks in multiples of 8 elements take the
+ * fast loads.  Sums are fp32; the rank products enter the second product as three 16-bit terms, which
+ * hold all 24 bits of the sum (fp16: of those down to 2^-16 of the token's largest, below that 2^-39
+ * of the largest).  How a sum is cut up follows the batch (its size, the declared groups, where a
+ * token's tile falls), so a token's last bits may change with its neighbours; the same batch gives the
+ * same bits.  Infinities in an adapter that a token uses may come out as NaN.  workspace:
+ * ugc_adapter_workspace bytes (0 for small batches, then NULL will do), 16-byte aligned, free again
+ * when the call's work is done. */
 #define UGC_ADAPTER_MAX_RANK 128
 int ugc_adapter_workspace(size_t n_tokens, int n_groups, size_t rank, size_t dim, size_t out_dim, size_t* bytes);
 int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base_stride, const void* x,
@@ -490,9 +495,10 @@ int ugc_adapter_add(int device_id, int elem_type, const void* base, int64_t base
                     const float* scale, const int32_t* offsets, const int32_t* order, size_t n_tokens,
                     int n_groups, size_t rank, size_t dim, size_t out_dim, void* out, int64_t out_stride,
                     void* workspace, size_t workspace_bytes, void* stream);
-/* The kernels of 16-bit adapters wait for their own copies and products; a wait that does not end within about
- * two seconds ends the kernel (what it has not stored by then stays as it was) and is counted per GPU.  The call has
- * returned long since: who wants to know reads this count, which synchronises; 0 on a sound machine. */
+/* The kernels of 16-bit adapters wait for their own copies and products; a wait that does not end
+ * within about two seconds ends the kernel (what it has not stored by then stays as it was) and is
+ * counted per GPU.  The call has returned long since: who wants to know reads this count, which
+ * synchronises; 0 on a sound machine. */
 int ugc_adapter_stalled(int device_id, uint32_t* count);
 
 /* -- introspection --------------------------------------------------------------------- */

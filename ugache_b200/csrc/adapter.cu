@@ -189,9 +189,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { retur
 // the cluster has a slice of dim and, later, of out_dim; the CTAs hand one another their partial rank products
 // through distributed shared memory.  `up` does not wait for those: a bulk copy brings the slice
 // (what fits) into shared memory meanwhile.  The matrix instructions take the columns of a product in any
-// order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.  4096 x 4096, bf16: one token of
-// rank 16 6.1 us (2.1 until its tile is known, 1.0 for the first product, 1.6 for the cluster's sums, 1.4 for the second), 48
-// tokens of 64 adapters 7.7 us (8.1 MB of matrices), of rank 64 15 us, of rank 128 31 us (66 MB, 2.1 TB/s).
+// order as long as both operands agree, so every lane loads 16 consecutive bytes of a row.  4096 x 4096, bf16: one token
+// of rank 16 6.5 us (about 2.1 until its tile is known, 1.0 for the first product, 1.6 for the cluster's sums, 1.4 for
+// the second), 48 tokens of 64 adapters 8.5 us (8.1 MB of matrices), of rank 64 17 us, of rank 128 33 us (66 MB, 2.0 TB/s).
 
 constexpr int kMostCluster = 8;
 
@@ -502,8 +502,8 @@ __global__ void __launch_bounds__(kBlock, RP <= 16 ? 4 : RP <= 32 ? 3 : 2) adapt
 // ------------------------------------------------------------------------------------
 // The matrix units have no fp32 products, so these are fused multiply-adds, 16 tokens a cluster as above: x goes
 // through shared memory 256 columns at a time, a warp has a rank and all tokens; then a thread has an output and all
-// tokens.  Bound by its instructions: 48 tokens of 64 adapters of rank 16 (4096 x 4096) take 28 us, 16,384 of 24 of
-// rank 64 1.56 ms (17 GFLOP; 3.2 ms with every sum shuffled alone and `up` read an element at a time).
+// tokens.  Bound by its instructions: 48 tokens of 64 adapters of rank 16 (4096 x 4096) take 27 us, 16,384 of 24 of
+// rank 64 1.55 ms (17 GFLOP; 3.2 ms with every sum shuffled alone and `up` read an element at a time).
 
 constexpr int kF32Columns = 256;
 
@@ -613,15 +613,15 @@ __global__ void __launch_bounds__(kBlock) adapter_f32_kernel(AdapterParams p) {
 // ------------------------------------------------------------------------------------
 // Two launches.  The first multiplies the tiles' rows of x with their adapters' `down` and leaves fp32
 // partial sums in the workspace; the second adds those up, splits them into three 16-bit terms and multiplies
-// them with `up`, adding `base` on the way out.  In both a tile is so many steps of 64 columns, the tiles of the
+// them with `up`, adding `base` on the way out.  In both a tile is so many steps of 128 columns, the tiles of the
 // batch stand one behind the other, and every CTA of a full GPU takes the same number of consecutive
 // steps, so that no number of tiles leaves part of the GPU idle; where a CTA's run starts or ends inside a tile
 // of the first product, the tile has one more partial sum.
 // Steps go through a ring of stages in shared memory: four warps copy (token rows lie anywhere, so 16
 // bytes a thread), one thread issues the matrix instructions, the other warps take the products out of
-// tensor memory.  HBM bounds it, through the bytes that the ring keeps in flight: 4096 x 4096, bf16, 16,384 tokens of 24
-// adapters of rank 16 / 64 / 128 take 80 / 89 / 119 us (62 / 65 / 69 at the rate of a plain copy), 65,536 of rank 64
-// 305 (250); with two stages less 90 at rank 16.
+// tensor memory.  HBM bounds it, through the bytes that the ring keeps in flight, and from rank 64 on the shared memory
+// that the products read: 4096 x 4096, bf16, 16,384 tokens of 24 adapters of rank 16 / 64 / 128 take 82 / 91 / 122 us (62 /
+// 65 / 69 at the rate of a plain copy), 65,536 of rank 64 318 to 328 (250); with two stages less 90 at rank 16.
 //
 // Operands lie in shared memory in rows of 128 bytes whose 16-byte pieces are exchanged by row (piece c
 // of row r at c ^ (r % 8)), as the matrix unit reads them: a line of global memory is a line there, and
@@ -957,9 +957,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     adapter_up_kernel(AdapterParams p, const float* __restrict__ inner, BigShare down_share, BigShare share) {
   using S = BigShape<RP>;
   constexpr int kStages = S::kUpStages, kColumns = 2 * kStep;
-  // pieces a thread takes out at once: with two stages the ring waits for them (rank 128: 16,384 prompts 119 us against
-  // 133 with four), with more the registers count
-  constexpr int kWide = kStages == 2 ? 8 : 4;
+  constexpr int kWide = 4;  // pieces a thread takes out at once; with eight rank 128 is no faster and rank 64 slower (92 us)
   extern __shared__ unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kStages], drained[kStages], product[2], taken[2], terms, tops;
   __shared__ uint32_t tmem_slot;
@@ -1188,13 +1186,13 @@ cudaError_t adapter_launch(const AdapterParams& p, bool vector, cudaStream_t str
   auto kern = vector ? adapter_kernel<E, RP, true> : adapter_kernel<E, RP, false>;
   constexpr uint32_t kSms = 148;
   const uint32_t tiles = small_tiles(p);
-  // Clusters of 8 are the shorter chain, of 4 the less work a tile: 64 tiles of rank 16 (4096 x 4096) 10.7 against 13.3 us,
-  // 128 tiles 15.6 against 12.8.
+  // Clusters of 8 are the shorter chain, of 4 the less work a tile: 64 tokens of 63 adapters of rank 16 (4096 x 4096) 9.9
+  // against 11.0 us, 128 of 127 18.5 against 14.4.
   const bool few = tiles * kMostCluster <= kSms * 9 / 2;
   const uint32_t cluster = few ? kMostCluster : kMostCluster / 2;
   // CTAs an SM, by shared memory: as few as hold the batch, so that they spread over all SMs (packed onto few
-  // of them 30 tiles took 9.9 us instead of 8.5), and of small clusters at most three (mixed prompts of 200 adapters 18.7 us
-  // with four, 16.4 with three).  What is left of it holds `up`.
+  // of them 30 tiles took 9.9 us instead of 8.5), and of small clusters at most three (1111 tokens of 200 adapters 30.2 us
+  // with four, 28.9 with three).  What is left of it holds `up`.
   constexpr uint32_t kMost = RP <= 32 ? 3 : 2;
   const uint32_t per_sm = std::min((tiles * cluster + kSms - 1) / kSms, few && RP <= 16 ? 4 : kMost);
   const uint32_t budget = std::min(216u * 1024 / per_sm, kMostShared);
@@ -1228,9 +1226,10 @@ BigSplit big_split(uint32_t n_tokens, uint32_t n_groups, uint32_t rank, uint32_t
 }
 
 // Tiles of 128 or of 16 tokens.  Against a tile of 16, one of 128 reads an adapter's matrices an eighth as often
-// but has a longer chain and two launches; what the former costs grows with tokens x rank.  Measured, 4096 x 4096, 16 | 128 a tile, us:
-// rank 16: 2048 tokens of 8 adapters 20.9 | 22.4, 4096 of 8 39.7 | 27.5, 4096 of 128 50 | 48, 4096 of 256 46 | 57;
-// rank 64: 256 of 8 14 | 19, 1024 of 32 46 | 30, 1024 of 64 47 | 29; rank 128: 256 of 8 24 | 29, 512 of 8 44 | 34.
+// but has a longer chain and two launches; what the former costs grows with tokens x rank.  Measured, 4096 x 4096,
+// inputs beyond the L2, 16 | 128 a tile, us: rank 16: 4096 tokens of 8 adapters 50 | 28, of 128 55 | 62, of 256 65 | 111; rank 64:
+// 256 of 8 15 | 21, 640 of 8 28 | 21, 1024 of 32 48 | 33, of 64 52 | 42; rank 128: 256 of 8 29 | 28, 320 of 8 29 | 28, 512 of 8 48 | 28.
+// Near the borders the two are close, or lie a little to either side (rank 16: 2048 of 8 32 | 23; 26 | 22 from the L2).
 bool big_batch(uint32_t n_tokens, uint32_t n_groups, uint32_t rank) {
   const unsigned long long work = (unsigned long long)n_tokens * padded_rank(rank);
   return work >= 40960 && work >= 512ull * n_groups;

@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kRowsBlock) spread_kernel(RouteRows p, uint32_
 }
 
 // A thread sums PIECES pieces of one token's row over its choices, in their order, in fp32: FLIGHT choices and
-// all pieces are on their way at once.  Bound by the bytes in flight: 32,768 tokens of 4 rows of 8 KiB 213 us (6.3 TB/s) with
+// all pieces are on their way at once.  Bound by the bytes in flight: 32,768 tokens of 4 rows of 8 KiB 220 us (6.1 TB/s) with
 // 4 x 2, 249 with 4 x 1, 292 with 4 x 4 (registers); two rows of 32 KiB 120 us with 2 x 4, 167 with 4 x 1.
 template <typename E, bool WEIGHTED, int FLIGHT, int PIECES>
 __global__ void __launch_bounds__(kRowsBlock) gather_kernel(RouteRows p, uint32_t pieces) {

@@ -398,10 +398,13 @@ def route_combine_grad(dy, plan, weights=None, rows=None, drows=None, stream=Non
 
 def adapter_add(base, x, down, up, plan, scale=None, out=None, stream=None):
     """``out[t] = base[t] + scale[a] * (x[t] @ down[a].T) @ up[a].T`` with ``a`` the adapter of token ``t`` in
-    ``plan`` (one id a token); tokens without one: ``base[t]``.  base ``[T, out_dim]`` (what the shared projection gave),
-    x ``[T, dim]``, down ``[adapters, rank, dim]``, up ``[adapters, out_dim, rank]``: float16 or bfloat16 (float32 is
-    taken, without the matrix units); scale float32 ``[adapters]``.  ``out`` may be ``base``.  Adapters kept as rows of a cache: ``down`` and ``up`` are views of the
-    rows of ``Cache.lookup_unique`` (of the batch's requests, 1024 at a time) and its ``inverse`` gives the ids of the plan."""
+    ``plan`` (one id a token); tokens without one: ``base[t]``.  base ``[T, out_dim]`` (what the shared
+    projection gave), x ``[T, dim]``, down ``[adapters, rank, dim]``, up ``[adapters, out_dim, rank]``: float16
+    or bfloat16 (float32 is taken, without the matrix units); scale float32 ``[adapters]``.  ``out`` may be
+    ``base``.  The matrices of an adapter have to be dense, adapters may lie any distance apart; what comes
+    otherwise (``up`` transposed, one adapter expanded) is copied whole in every call.  Adapters kept as rows
+    of a cache: ``down`` and ``up`` are views of the rows of ``Cache.lookup_unique`` (of the batch's requests,
+    1024 at a time) and its ``inverse`` gives the ids of the plan."""
     return (_lib._fast or _lib.fast()).adapter_add(base, x, down, up, plan.offsets, plan.order, scale, out, stream)
 
 
